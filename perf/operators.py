@@ -94,7 +94,8 @@ def work(case):
         return {"bytes": 12 * r * k + (8 * r * k if case["acc"] else 4 * r * c), "flops": 0}
     if case["op"] == "distill":
         r, c, k = case["rows"], case["cols"], case["k"]
-        read = 4 * r * c + 12 * r * k + (4 * r if case["weights"] else 0)
+        real = r * 15 // 16 if case["weights"] else r  # rows that are no padding: only their logits are needed
+        read = 4 * real * c + 12 * real * k + (4 * r if case["weights"] else 0)
         if case["dir"] == "fwd":
             return {"bytes": read + 12 * r + 4, "flops": 4 * r * c}
         grad = 4 * r * c * (2 if case["acc"] else 1)
@@ -259,7 +260,7 @@ def _plain_distill(s):
             row_loss = torch.where(s["w"] != 0, row_loss, 0.0)
         out.update(row_loss=row_loss, loss=(row_loss.double() * w).sum().float().reshape(1))
         if s["dir"] == "fwd":
-            out["stats"] = stats
+            out["stats"] = stats if s["w"] is None else torch.where(s["w"].unsqueeze(1) != 0, stats, 0.0)
     if s["dir"] != "fwd":
         d = ((x - stats[:, :1]) / temp - stats[:, 1:]).exp_()
         d.scatter_add_(1, at, -q)
@@ -449,7 +450,7 @@ def _exact_distill(s):
             part["loss"] = (w * kl).sum().reshape(1)
         if s["dir"] == "fwd":
             top = x.max(dim=1).values
-            part["stats"] = torch.stack([top, torch.logsumexp(x / temp, dim=1) - top / temp], dim=1)
+            part["stats"] = torch.stack([top, torch.logsumexp(x / temp, dim=1) - top / temp], dim=1) * (w != 0).unsqueeze(1)
         if s["dir"] != "fwd":
             part["grad"] = temp * w.unsqueeze(1) * (log_p.exp() - whole)
             if s["acc"]:
