@@ -1,7 +1,7 @@
 """ctypes loader for libzg_hip.so.
 
-Prototypes are taken from include/zg_hip.h itself, so the Python side cannot drift from the C ABI:
-every `zg_hip_*` declaration in the header becomes a bound function with argument and return types.
+Prototypes are taken from include/zg_hip.h and include/zg_hip_topk.h themselves, so the Python side cannot drift from
+the C ABI: every `zg_hip_*` declaration in the headers becomes a bound function with argument and return types.
 Loading fails loudly when the library is missing; there is no CPU fallback.
 """
 from __future__ import annotations
@@ -12,6 +12,7 @@ from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
 HEADER = PKG_DIR.parent / "include" / "zg_hip.h"
+TOPK_HEADER = PKG_DIR.parent / "include" / "zg_hip_topk.h"  # the operators built on the k largest of a row
 LIB_PATH = PKG_DIR / "libzg_hip.so"
 
 _SCALARS = {
@@ -74,7 +75,7 @@ class Library:
             )
         self.path = Path(path)
         self.cdll = ctypes.CDLL(str(path))
-        self.protos = parse_header()
+        self.protos = {**parse_header(), **parse_header(TOPK_HEADER)}
         for name, (restype, params) in self.protos.items():
             fn = getattr(self.cdll, name)  # AttributeError here means the .so lacks a declared symbol
             fn.restype = restype

@@ -24,6 +24,7 @@ extern std::atomic<unsigned long long> launches_issued;  // process-wide: contex
 #include <vector>
 
 #include "../../include/zg_hip.h"
+#include "../../include/zg_hip_topk.h"
 
 #define ZG_API extern "C" __attribute__((visibility("default")))
 
@@ -433,6 +434,28 @@ inline size_t ceil_div_sz(size_t a, size_t b) {
 inline bool aligned16(const void* p) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }
+// Whether two operands share a byte.
+inline bool ranges_overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const char *x = (const char*)a, *y = (const char*)b;
+    return a && b && a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+// a * b, or SIZE_MAX where that does not fit: what an argument check compares with
+inline size_t mul_sat(size_t a, size_t b) {
+    size_t r;
+    return __builtin_mul_overflow(a, b, &r) ? (size_t)-1 : r;
+}
+
+// Makes the context's device current for the length of a call (a caller may have another one current).
+struct DeviceGuard {
+    int before = -1;
+    explicit DeviceGuard(const zg_hip_ctx* ctx) {
+        int now = -1;
+        if (hipGetDevice(&now) == hipSuccess && now != ctx->device && hipSetDevice(ctx->device) == hipSuccess) before = now;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
 
 }  // namespace zg
 

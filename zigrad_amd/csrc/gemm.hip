@@ -222,7 +222,60 @@ struct GemmArgs {
     const float* bias;
     const float* gate;
     int relu;
+    // Experts' products (kernels with GROUP != 0): expert e's rows are offsets[e] .. offsets[e + 1] - 1 of n_rows
+    const uint64_t* offsets;
+    unsigned n_experts;
+    size_t n_rows;
 };
+
+// The rows of expert e, whatever the offsets hold: inside [0, n_rows), none when the range ends before it begins.
+__device__ __forceinline__ void expert_range(const uint64_t* offsets, unsigned e, size_t n_rows, uint32_t& first, uint32_t& count) {
+    const uint64_t lo = offsets[e] < n_rows ? offsets[e] : n_rows, hi = offsets[e + 1] < n_rows ? offsets[e + 1] : n_rows;
+    first = (uint32_t)lo;
+    count = hi > lo ? (uint32_t)(hi - lo) : 0u;
+}
+// The tile_m-th tile of BM rows over all experts' rows, each expert's own tiles: which expert, its rows, the tile within.
+// Every wave of the workgroup finds it by itself, 64 experts at a time, lane l holding expert base + l.
+struct ExpertTile {
+    unsigned e, tile, first, count;
+};
+__device__ __forceinline__ unsigned wave_scan(unsigned v, int lane) {  // inclusive sum over the lanes
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const unsigned o = (unsigned)__shfl_up((int)v, d, kWave);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+template <int BM>
+__device__ __forceinline__ unsigned expert_tiles(const uint64_t* offsets, unsigned n_experts, size_t n_rows, int lane) {
+    unsigned total = 0;
+    for (unsigned base = 0; base < n_experts; base += kWave) {
+        uint32_t first = 0, count = 0;
+        if (base + lane < n_experts) expert_range(offsets, base + lane, n_rows, first, count);
+        const unsigned incl = wave_scan((count + BM - 1) / BM, lane);
+        total += (unsigned)__builtin_amdgcn_readlane((int)incl, kWave - 1);
+    }
+    return total;
+}
+template <int BM>
+__device__ __forceinline__ ExpertTile find_expert_tile(const uint64_t* offsets, unsigned n_experts, size_t n_rows, unsigned tile_m,
+                                                       int lane) {
+    unsigned before = 0;
+    for (unsigned base = 0; base < n_experts; base += kWave) {
+        uint32_t first = 0, count = 0;
+        if (base + lane < n_experts) expert_range(offsets, base + lane, n_rows, first, count);
+        const unsigned tiles = (count + BM - 1) / BM, incl = wave_scan(tiles, lane) + before;
+        const uint64_t hit = __ballot(tile_m >= incl - tiles && tile_m < incl);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            return {base + l, tile_m - (unsigned)__builtin_amdgcn_readlane((int)(incl - tiles), l),
+                    (unsigned)__builtin_amdgcn_readlane((int)first, l), (unsigned)__builtin_amdgcn_readlane((int)count, l)};
+        }
+        before = (unsigned)__builtin_amdgcn_readlane((int)incl, kWave - 1);
+    }
+    return {0, 0, 0, 0};  // not reached: the caller has checked tile_m against expert_tiles()
+}
 
 // the epilogue extras on one value (the rounding of the separate add / relu / mask kernels: one IEEE add, selects)
 __device__ __forceinline__ float gemm_extras(float v, bool has_bias, float bias, bool relu) {
@@ -265,7 +318,9 @@ __device__ __forceinline__ void tile_coords(unsigned id, unsigned tiles_m, unsig
 // MODE 2 (checked): every load checked and zero-filled; only for leading dimensions beyond 32-bit byte offsets.
 // TAILS: the launch has its tail in pieces (GemmArgs::tail_part); instantiated for the 128 x 128 and 64 x 64 tiles only
 // (the 256 x 128 kernels' register budget has no room for it, and the planner never asks them).
-template <int BM, int BN, bool A_KMAJOR, bool B_KMAJOR, int MODE, bool TAILS = false>
+// GROUP (with MODE 1): the experts' products.  1: the rows of A and C belong to experts by ranges, B and the bias to the
+// expert: the workgroup's tile is the id-th of all experts' tiles.  2: k runs over the rows of expert blockIdx.z.
+template <int BM, int BN, bool A_KMAJOR, bool B_KMAJOR, int MODE, bool TAILS = false, int GROUP = 0>
 __global__ __launch_bounds__(kGemmThreads) void gemm_kernel(GemmArgs g) {
     constexpr bool SAFE = MODE == 2;
     constexpr int BK = kBK;
@@ -296,6 +351,41 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_kernel(GemmArgs g) {
             piece_id = blockIdx.x - g.tail_first;
             split = piece_id % g.tail_splits;
             tile_coords(g.tail_first + piece_id / g.tail_splits, g.tiles_m, g.tiles_n, tm, tn);
+        }
+    } else if constexpr (GROUP == 1) {
+        // tiles there really are, dealt to the XCDs in contiguous runs; the grid has room for the most there can be
+        const unsigned tiles_m = expert_tiles<BM>(g.offsets, g.n_experts, g.n_rows, threadIdx.x & 63);
+        const unsigned total = tiles_m * g.tiles_n, run = (total + 7) / 8;
+        const unsigned id = (blockIdx.x & 7u) * run + (blockIdx.x >> 3);
+        if ((blockIdx.x >> 3) >= run || id >= total) return;
+        tile_coords(id, tiles_m, g.tiles_n, tm, tn);
+        const ExpertTile t = find_expert_tile<BM>(g.offsets, g.n_experts, g.n_rows, tm, threadIdx.x & 63);
+        tm = t.tile;
+        g.A += (size_t)t.first * g.lda;
+        g.C += (size_t)t.first * g.ldc;
+        if (g.gate) g.gate += (size_t)t.first * g.ldc;
+        if (g.bias) g.bias += (size_t)t.e * g.N;
+        g.M = t.count;
+        g.B += (size_t)t.e * g.b_chunk;
+        z = 0;
+    } else if constexpr (GROUP == 2) {
+        uint32_t first, count;
+        expert_range(g.offsets, blockIdx.z, g.n_rows, first, count);
+        first = (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
+        count = (uint32_t)__builtin_amdgcn_readfirstlane((int)count);
+        tile_coords(xcd_contiguous(blockIdx.x, g.tiles_m * g.tiles_n), g.tiles_m, g.tiles_n, tm, tn);
+        g.K = count;
+        g.A += (size_t)first * g.lda;
+        g.B += (size_t)first * g.ldb;
+        if (count == 0) {  // an expert without rows: C is left, or zero
+            if (g.beta == 0.f) {
+                float* C = g.C + z * g.c_chunk;
+                for (unsigned i = threadIdx.x; i < BM * BN; i += kGemmThreads) {
+                    const size_t row = (size_t)tm * BM + i / BN, col = (size_t)tn * BN + i % BN;
+                    if (row < g.M && col < g.N) C[row * g.ldc + col] = 0.f;
+                }
+            }
+            return;
         }
     } else {
         const unsigned per_batch = g.tiles_m * g.tiles_n;
@@ -1426,6 +1516,9 @@ static GemmArgs gemm_args(const float* A, const float* B, float* C, size_t m, si
     g.tail_part = nullptr;
     g.c_vec = 0;
     g.bounded_tail = 0;
+    g.offsets = nullptr;
+    g.n_experts = 0;
+    g.n_rows = 0;
     return g;
 }
 
@@ -2463,6 +2556,139 @@ ZG_API int zg_hip_linear_bwd(zg_hip_ctx* ctx, const float* gy, const float* x, c
                              1, 1, 1, 0, 0, 0);
     }
     return launch_linear_bwd_small(ctx, gy, x, fan_in, w, fan_in, act_in, gw, 1.f, gb, 1.f, gx, batch, fan_in, fan_out);
+}
+
+namespace zg {
+// ------------------------------------------------------------------------------------------------
+// The experts' Linear layers: the staged kernels' edge mode with each expert's rows as a product of its own, found by the
+// workgroups from the offsets in device memory.
+// ------------------------------------------------------------------------------------------------
+constexpr size_t kExpertMaxDim = (size_t)1 << 21;  // leading dimensions whose tiles have 32-bit byte offsets
+
+static int expert_linear_check(const char* op, const uint64_t* offsets, size_t n_rows, size_t n_experts, size_t fan_in,
+                               size_t fan_out) {
+    ZG_REQUIRE(n_experts >= 1 && n_experts <= ZG_HIP_EXPERTS_MAX, "%s: %zu experts are not in 1 .. %d", op, n_experts,
+               (int)ZG_HIP_EXPERTS_MAX);
+    ZG_REQUIRE(n_rows < ((size_t)1 << 31), "%s: %zu rows", op, n_rows);
+    ZG_REQUIRE(fan_in < kExpertMaxDim && fan_out < kExpertMaxDim, "%s: a layer of %zu x %zu", op, fan_out, fan_in);
+    ZG_REQUIRE(offsets && ((uintptr_t)offsets & 7u) == 0, "%s: offsets are null or not on an 8-byte boundary", op);
+    return ZG_HIP_OK;
+}
+
+// C[rows of e] = A[rows of e] op(B_e) with the extras
+template <int BM, int BN, bool B_KMAJOR>
+static int launch_expert_rows(zg_hip_ctx* ctx, GemmArgs g) {
+    g.tiles_n = (unsigned)ceil_div_sz(g.N, BN);
+    const size_t most = g.n_rows / BM + (g.n_rows < g.n_experts ? g.n_rows : g.n_experts);  // tiles of rows there can be
+    const size_t blocks = (most * g.tiles_n + 7) / 8 * 8;
+    ZG_REQUIRE(blocks < 0x7fffffffull, "expert_linear: %zu workgroups", blocks);
+    constexpr size_t lds = 2 * (size_t)(Tile<BM, true>::ELEMS + Tile<BN, B_KMAJOR>::ELEMS) * sizeof(float);
+    hipLaunchKernelGGL((gemm_kernel<BM, BN, true, B_KMAJOR, 1, false, 1>), dim3((unsigned)blocks), dim3(kGemmThreads), lds,
+                       ctx->stream, g);
+    ZG_LAUNCH_CHECK();
+    return ZG_HIP_OK;
+}
+template <bool B_KMAJOR>
+static int expert_rows(zg_hip_ctx* ctx, const float* A, const float* B, float* C, const uint64_t* offsets, size_t n_rows,
+                       size_t n_experts, size_t n, size_t k, const float* bias, const float* gate, int relu) {
+    const GemmExtras ex{bias, gate, relu};
+    GemmArgs g = gemm_args(A, B, C, n_rows, n, k, 0, B_KMAJOR, k, B_KMAJOR ? k : n, n, 1.f, 0.f, 1, 1, 0, n * k, 0, &ex);
+    g.offsets = offsets;
+    g.n_experts = (unsigned)n_experts;
+    g.n_rows = n_rows;
+    g.split_tiles = ceil_div_sz(k, kBK);
+    g.c_vec = aligned16(C) && n % 4 == 0 && (!gate || aligned16(gate));
+    g.bounded_tail = !B_KMAJOR && n % 4 != 0;
+    return launch_expert_rows<64, 64, B_KMAJOR>(ctx, g);
+}
+// C_e (+)= A[rows of e]^T B[rows of e]
+template <int BM, int BN>
+static int launch_expert_weights(zg_hip_ctx* ctx, GemmArgs g) {
+    g.tiles_m = (unsigned)ceil_div_sz(g.M, BM);
+    g.tiles_n = (unsigned)ceil_div_sz(g.N, BN);
+    ZG_REQUIRE((size_t)g.tiles_m * g.tiles_n < 0x7fffffffull, "expert_linear_bwd: a layer of %zu x %zu", g.M, g.N);
+    constexpr size_t lds = 2 * (size_t)(Tile<BM, false>::ELEMS + Tile<BN, false>::ELEMS) * sizeof(float);
+    hipLaunchKernelGGL((gemm_kernel<BM, BN, false, false, 1, false, 2>), dim3(g.tiles_m * g.tiles_n, 1, g.n_experts),
+                       dim3(kGemmThreads), lds, ctx->stream, g);
+    ZG_LAUNCH_CHECK();
+    return ZG_HIP_OK;
+}
+
+// gb_e (+)= column sums of expert e's rows: 64 columns x 4 row-threads
+template <bool ACC>
+__global__ __launch_bounds__(256) void expert_bias_grad_kernel(const float* gy, float* gb, const uint64_t* offsets, size_t n_rows,
+                                                                size_t fan_out) {
+    __shared__ float part[4][64];
+    uint32_t first, count;
+    expert_range(offsets, blockIdx.y, n_rows, first, count);
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const size_t col = (size_t)blockIdx.x * 64 + tx;
+    float sum = 0.f;
+    if (col < fan_out)
+        for (uint32_t r = ty; r < count; r += 4) sum += gy[(size_t)(first + r) * fan_out + col];
+    part[ty][tx] = sum;
+    __syncthreads();
+    if (ty == 0 && col < fan_out) {
+        float* to = gb + (size_t)blockIdx.y * fan_out + col;
+        const float v = (part[0][tx] + part[1][tx]) + (part[2][tx] + part[3][tx]);
+        *to = ACC ? *to + v : v;
+    }
+}
+}  // namespace zg
+
+ZG_API int zg_hip_expert_linear_fwd(zg_hip_ctx* ctx, const float* x, const float* w, const float* bias, float* y,
+                                    const uint64_t* offsets, size_t n_rows, size_t n_experts, size_t fan_in, size_t fan_out,
+                                    int relu) {
+    ZG_CTX(ctx);
+    if (int rc = expert_linear_check("expert_linear_fwd", offsets, n_rows, n_experts, fan_in, fan_out)) return rc;
+    if (n_rows == 0 || fan_out == 0) return ZG_HIP_OK;
+    ZG_REQUIRE(fan_in >= 1, "expert_linear_fwd: no inputs");
+    ZG_REQUIRE(x && w && y, "expert_linear_fwd: null pointer");
+    const size_t y_bytes = n_rows * fan_out * 4;
+    ZG_REQUIRE(!ranges_overlap(y, y_bytes, x, n_rows * fan_in * 4) && !ranges_overlap(y, y_bytes, w, n_experts * fan_in * fan_out * 4) &&
+                   !ranges_overlap(y, y_bytes, bias, n_experts * fan_out * 4) && !ranges_overlap(y, y_bytes, offsets, (n_experts + 1) * 8),
+               "expert_linear_fwd: y overlaps an input");
+    DeviceGuard guard(ctx);
+    return expert_rows<true>(ctx, x, w, y, offsets, n_rows, n_experts, fan_out, fan_in, bias, nullptr, relu);
+}
+
+ZG_API int zg_hip_expert_linear_bwd(zg_hip_ctx* ctx, const float* gy, const float* x, const float* w, const float* act_in,
+                                    float* gw, float* gb, float* gx, const uint64_t* offsets, size_t n_rows, size_t n_experts,
+                                    size_t fan_in, size_t fan_out, int accumulate) {
+    ZG_CTX(ctx);
+    if (int rc = expert_linear_check("expert_linear_bwd", offsets, n_rows, n_experts, fan_in, fan_out)) return rc;
+    if (fan_out == 0 || fan_in == 0) return ZG_HIP_OK;
+    ZG_REQUIRE(gw && (n_rows == 0 || (gy && x && (!gx || w))), "expert_linear_bwd: null pointer");
+    const void* const ins[5] = {gy, x, gx ? w : nullptr, gx ? act_in : nullptr, offsets};
+    const size_t in_bytes[5] = {n_rows * fan_out * 4, n_rows * fan_in * 4, n_experts * fan_in * fan_out * 4, n_rows * fan_in * 4,
+                                (n_experts + 1) * 8};
+    void* const outs[3] = {gw, gb, gx};
+    const size_t out_bytes[3] = {n_experts * fan_in * fan_out * 4, n_experts * fan_out * 4, n_rows * fan_in * 4};
+    for (int o = 0; o < 3; o++) {
+        for (int i = 0; i < 5; i++)
+            ZG_REQUIRE(!ranges_overlap(outs[o], out_bytes[o], ins[i], in_bytes[i]), "expert_linear_bwd: an output overlaps an input");
+        for (int i = 0; i < o; i++)
+            ZG_REQUIRE(!ranges_overlap(outs[o], out_bytes[o], outs[i], out_bytes[i]), "expert_linear_bwd: two outputs overlap");
+    }
+    DeviceGuard guard(ctx);
+    // the weight gradient runs over no rows too: it writes zeros then
+    GemmArgs g = gemm_args(gy, x, gw, fan_out, fan_in, n_rows, 1, 0, fan_out, fan_in, fan_in, 1.f, accumulate ? 1.f : 0.f, 1, 1, 0, 0,
+                           fan_out * fan_in, nullptr);
+    g.offsets = offsets;
+    g.n_experts = (unsigned)n_experts;
+    g.n_rows = n_rows;
+    g.split_tiles = (size_t)1 << 28;  // all of k
+    g.c_vec = aligned16(gw) && fan_in % 4 == 0;
+    g.bounded_tail = fan_out % 4 != 0 || fan_in % 4 != 0;
+    if (int rc = launch_expert_weights<64, 64>(ctx, g)) return rc;
+    if (gb) {
+        const dim3 grid((unsigned)ceil_div_sz(fan_out, 64), (unsigned)n_experts);
+        if (accumulate) hipLaunchKernelGGL(expert_bias_grad_kernel<true>, grid, dim3(256), 0, ctx->stream, gy, gb, offsets, n_rows, fan_out);
+        else hipLaunchKernelGGL(expert_bias_grad_kernel<false>, grid, dim3(256), 0, ctx->stream, gy, gb, offsets, n_rows, fan_out);
+        ZG_LAUNCH_CHECK();
+    }
+    if (!gx || n_rows == 0) return ZG_HIP_OK;
+    return expert_rows<false>(ctx, gy, w, gx, offsets, n_rows, n_experts, fan_in, fan_out, nullptr, act_in, 0);
 }
 
 ZG_API int zg_hip_bmm_acc(zg_hip_ctx* ctx, const float* A, const uint64_t* A_shape, const float* B,

@@ -544,6 +544,96 @@ class HipDevice:
     def _op_mse_fwd(self, pred, target, loss): self._call("zg_hip_mse_fwd", pred.ptr, target.ptr, pred.n, loss.ptr)
     def _op_mse_bwd(self, pred, target, grad): self._call("zg_hip_mse_bwd", pred.ptr, target.ptr, grad.ptr, pred.n)
 
+    # operators built on the k largest of a row (include/zg_hip_topk.h)
+    @staticmethod
+    def _need(op, **sizes):
+        """Buffers that must hold at least so many elements: {name: (buffer, elements)}; index arrays are 64-bit."""
+        for name, (buf, n) in sizes.items():
+            if buf is None:
+                continue
+            want = U64 if name in ("indices", "experts", "offsets", "slots") else F32
+            if buf.dtype != want:
+                raise TypeError(f"{op}: {name} must be {want}, not {buf.dtype}")
+            if buf.n < n:
+                raise ValueError(f"{op}: {name} holds {buf.n} elements, {n} are needed")
+
+    def _op_topk_fwd(self, x, values, indices, rows, cols, k):
+        """The k largest of each row in descending order, and their columns; the lowest column first among equals."""
+        self._need("topk_fwd", x=(x, rows * cols), values=(values, rows * k), indices=(indices, rows * k))
+        self._call("zg_hip_topk_fwd", x.ptr, values.ptr, indices.ptr, rows, cols, k)
+
+    def _op_topk_bwd(self, indices, y_g, x_g, rows, cols, k, accumulate=True):
+        self._need("topk_bwd", indices=(indices, rows * k), y_g=(y_g, rows * k), x_g=(x_g, rows * cols))
+        self._call("zg_hip_topk_bwd", indices.ptr, y_g.ptr, x_g.ptr, rows, cols, k, int(bool(accumulate)))
+
+    def _op_distill_fwd(self, logits, teacher, indices, stats, row_loss, loss, rows, cols, k, temperature=1.0, weights=None):
+        """Loss of a student's logits against a teacher's k largest; weights (one per row) may be None: the mean."""
+        self._need("distill_fwd", logits=(logits, rows * cols), teacher=(teacher, rows * k), indices=(indices, rows * k),
+                   weights=(weights, rows), stats=(stats, 2 * rows), row_loss=(row_loss, rows), loss=(loss, 1))
+        self._call("zg_hip_distill_fwd", logits.ptr, teacher.ptr, indices.ptr, weights.ptr if weights is not None else None,
+                   stats.ptr, row_loss.ptr, loss.ptr, rows, cols, k, temperature)
+
+    def _op_distill_bwd(self, logits, teacher, indices, stats, grad, rows, cols, k, temperature=1.0, weights=None,
+                        accumulate=True):
+        self._need("distill_bwd", logits=(logits, rows * cols), teacher=(teacher, rows * k), indices=(indices, rows * k),
+                   weights=(weights, rows), stats=(stats, 2 * rows), grad=(grad, rows * cols))
+        self._call("zg_hip_distill_bwd", logits.ptr, teacher.ptr, indices.ptr, weights.ptr if weights is not None else None,
+                   stats.ptr, grad.ptr, rows, cols, k, temperature, int(bool(accumulate)))
+
+    def _op_distill_fwd_bwd(self, logits, teacher, indices, stats, row_loss, loss, grad, rows, cols, k, temperature=1.0,
+                            weights=None, accumulate=True):
+        self._need("distill_fwd_bwd", logits=(logits, rows * cols), teacher=(teacher, rows * k), indices=(indices, rows * k),
+                   weights=(weights, rows), stats=(stats, 2 * rows), row_loss=(row_loss, rows), loss=(loss, 1),
+                   grad=(grad, rows * cols))
+        self._call("zg_hip_distill_fwd_bwd", logits.ptr, teacher.ptr, indices.ptr,
+                   weights.ptr if weights is not None else None, stats.ptr, row_loss.ptr, loss.ptr, grad.ptr, rows, cols, k,
+                   temperature, int(bool(accumulate)))
+
+    def _op_expert_sort(self, experts, offsets, slots, n_experts):
+        """Order the entries by expert: slots[i] = entry i's place (2^64 - 1: dropped), offsets = the experts' first places."""
+        self._need("expert_sort", experts=(experts, 0), offsets=(offsets, n_experts + 1), slots=(slots, experts.n))
+        self._call("zg_hip_expert_sort", experts.ptr, offsets.ptr, slots.ptr, experts.n, n_experts)
+
+    def _op_expert_dispatch(self, x, slots, y, n_tokens, k, width):
+        self._need("expert_dispatch", x=(x, n_tokens * width), slots=(slots, n_tokens * k), y=(y, n_tokens * k * width))
+        self._call("zg_hip_expert_dispatch", x.ptr, slots.ptr, y.ptr, n_tokens, k, width)
+
+    def _op_expert_dispatch_bwd(self, y_g, slots, x_g, n_tokens, k, width, accumulate=True):
+        self._need("expert_dispatch_bwd", y_g=(y_g, n_tokens * k * width), slots=(slots, n_tokens * k),
+                   x_g=(x_g, n_tokens * width))
+        self._call("zg_hip_expert_dispatch_bwd", y_g.ptr, slots.ptr, x_g.ptr, n_tokens, k, width, int(bool(accumulate)))
+
+    def _op_expert_combine(self, y, slots, weights, out, n_tokens, k, width):
+        self._need("expert_combine", y=(y, n_tokens * k * width), slots=(slots, n_tokens * k), weights=(weights, n_tokens * k),
+                   out=(out, n_tokens * width))
+        self._call("zg_hip_expert_combine", y.ptr, slots.ptr, weights.ptr, out.ptr, n_tokens, k, width)
+
+    def _op_expert_combine_bwd(self, out_g, slots, weights, n_tokens, k, width, y=None, y_g=None, weights_g=None):
+        """y_g or weights_g may be None (not computed); y is read for weights_g only."""
+        opt = lambda b: b.ptr if b is not None else None
+        self._need("expert_combine_bwd", out_g=(out_g, n_tokens * width), slots=(slots, n_tokens * k),
+                   weights=(weights, n_tokens * k), y=(y, n_tokens * k * width), y_g=(y_g, n_tokens * k * width),
+                   weights_g=(weights_g, n_tokens * k))
+        self._call("zg_hip_expert_combine_bwd", out_g.ptr, opt(y), slots.ptr, weights.ptr, opt(y_g), opt(weights_g), n_tokens,
+                   k, width)
+
+    def _op_expert_linear_fwd(self, x, w, bias, y, offsets, n_rows, n_experts, fan_in, fan_out, relu):
+        """y = act(x . w_e^T + bias_e) for each expert's rows; bias may be None."""
+        self._need("expert_linear_fwd", x=(x, n_rows * fan_in), w=(w, n_experts * fan_out * fan_in),
+                   bias=(bias, n_experts * fan_out), y=(y, n_rows * fan_out), offsets=(offsets, n_experts + 1))
+        self._call("zg_hip_expert_linear_fwd", x.ptr, w.ptr, bias.ptr if bias is not None else None, y.ptr, offsets.ptr, n_rows,
+                   n_experts, fan_in, fan_out, int(bool(relu)))
+
+    def _op_expert_linear_bwd(self, gy, x, w, act_in, gw, gb, gx, offsets, n_rows, n_experts, fan_in, fan_out,
+                              accumulate=True):
+        """gw_e (+)= gy_e^T . x_e; gb_e (+)= column sums (None: none); gx = gy . w_e, zeroed where act_in <= 0 (None: none)."""
+        opt = lambda b: b.ptr if b is not None else None
+        self._need("expert_linear_bwd", gy=(gy, n_rows * fan_out), x=(x, n_rows * fan_in), w=(w, n_experts * fan_out * fan_in),
+                   act_in=(act_in, n_rows * fan_in), gw=(gw, n_experts * fan_out * fan_in), gb=(gb, n_experts * fan_out),
+                   gx=(gx, n_rows * fan_in), offsets=(offsets, n_experts + 1))
+        self._call("zg_hip_expert_linear_bwd", gy.ptr, x.ptr, opt(w), opt(act_in), gw.ptr, opt(gb), opt(gx), offsets.ptr,
+                   n_rows, n_experts, fan_in, fan_out, int(bool(accumulate)))
+
     # optimizers
     def _op_sgd_step(self, param, grad, lr, clip, max_norm, delta):
         self._call("zg_hip_sgd_step", param.ptr, grad.ptr, param.n, lr, int(clip), max_norm, delta)
