@@ -28,7 +28,7 @@ enum {
 /* ---------------------------------------------------------------------------------------------
  * selection.  values[r, :] = the k largest of x[r, :] in descending order, indices[r, :] their columns.  Equal values
  * (+0 and -0 are equal) come in the order of their columns; a NaN counts as larger than any number, as in zg_hip_max_fwd.
- * 1 <= k <= min(cols, ZG_HIP_TOPK_MAX_K), cols < 2^32; no rows: nothing to do.  Few long rows use the workspace.
+ * 1 <= k <= min(cols, ZG_HIP_TOPK_MAX_K), cols < 2^31; no rows: nothing to do.  Few long rows use the workspace.
  * ------------------------------------------------------------------------------------------- */
 int zg_hip_topk_fwd(zg_hip_ctx *ctx, const float *x, float *values, uint64_t *indices, size_t rows, size_t cols, size_t k);
 /* x_g[r, indices[r, j]] += y_g[r, j]; accumulate == 0: x_g is written, zero in every place that was not chosen.  Indices that
@@ -48,7 +48,7 @@ int zg_hip_topk_bwd(zg_hip_ctx *ctx, const uint64_t *indices, const float *y_g, 
  * 0, whatever its logits hold) when its weight is 0, when it has no teacher logit above -inf, or when all its logits
  * are -inf.  A class of p = 0 that the teacher wants (q > 0) makes the row's loss infinite and leaves its gradient finite.
  * stats[r, :] = { max_c logits, log sum_c exp((logits - max) / temperature) }, {-inf, 0} for a row whose logits are all -inf,
- * {0, 0} for a row of weight 0 (its logits are not read): what zg_hip_distill_bwd needs of the row.  temperature > 0 and finite; cols < 2^32.  As with the other
+ * {0, 0} for a row of weight 0 (its logits are not read): what zg_hip_distill_bwd needs of the row.  temperature > 0 and finite; cols < 2^31.  As with the other
  * losses the forward calls refuse an empty matrix and the backward does nothing on one.  Rows longer than a workgroup's
  * share of a small batch use the workspace.
  * ------------------------------------------------------------------------------------------- */

@@ -13,43 +13,271 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 // Key of an element of a row: equal values order by column, the lower column being the larger key, so no two are equal.
 __device__ __forceinline__ uint64_t element_key(uint32_t key, uint32_t col) { return ((uint64_t)key << 32) | (uint32_t)~col; }
 
-struct MaxKey {
-    using Acc = uint64_t;
-    static __device__ __forceinline__ Acc init() { return 0; }
-    static __device__ __forceinline__ Acc combine(Acc a, Acc b) { return a > b ? a : b; }
-    static __device__ __forceinline__ Acc shfl_xor(Acc a, int m) { return (Acc)__shfl_xor((unsigned long long)a, m, kWave); }
+// The float whose key this is; numbers that are no float's key come out as NaN.
+__device__ __forceinline__ float key_value(uint32_t key) {
+    return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
+
+constexpr int kMaxK = ZG_HIP_TOPK_MAX_K;
+
+// ------------------------------------------------------------------------------------------------
+// Selection.  NT threads (a wave, or a workgroup of four) own a row and read it once:
+//   * the first NT x 4 x VPT values are held in registers as 4 NT groups, and the k-th largest of the groups' maxima is a
+//     lower bound of the row's k-th largest value (k groups hold a value at least that large each).  It is found bit by
+//     bit from the top, counting with ballots, and only to 16 bits: a bound that is a little low lets a few more through;
+//   * values that reach the bound become candidates in LDS as 64-bit keys (value, then column), about k of them among the
+//     first values and k / (4 NT VPT) of the rest of the row.  A thread looks at its single values only when their maximum
+//     reaches the bound, so the row is read at the memory's rate;
+//   * with more than kRankMost candidates the k largest are cut out by a radix selection over their keys (eight bits at a
+//     time, as many digits as it takes to tell them apart), which also raises the bound for the rest of the row;
+//   * a candidate's place in the result is the number of larger keys, which every thread counts for its own candidates.
+// Keys are unique, so neither the order in which candidates arrive nor the variant taken changes the result.
+// When a stretch of the row brings more candidates than LDS has room for (rows in rising order, rows of few different values) the
+// row is read again in pieces that fit whatever they hold (select_slowly).
+// ------------------------------------------------------------------------------------------------
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes at any 4-byte alignment
+
+template <int NT>
+struct Select {
+    static constexpr int kWaves = NT / kWave;
+    static constexpr int kCap = NT == kWave ? 1024 : 4096;
+    static constexpr uint32_t kRankMost = 384;
+    uint64_t key[kCap + 2];
+    uint32_t hist[256];
+    uint32_t count[2][kWaves];
+    uint32_t n;  // candidates asked for; those past kCap found no room
 };
 
-__global__ __launch_bounds__(kBlock) void topk_rounds_kernel(const float* x, float* values, uint64_t* indices, size_t rows,
-                                                              size_t cols, size_t k) {
-    __shared__ uint64_t smem[kBlock / kWave];
-    __shared__ uint64_t best;
-    for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        uint64_t below = ~(uint64_t)0;
-        for (size_t j = 0; j < k; j++) {
-            uint64_t m = 0;
-            for (size_t c = threadIdx.x; c < cols; c += kBlock) {
-                const uint64_t key = element_key(order_key(x[r * cols + c]), (uint32_t)c);
-                if (key < below && key > m) m = key;
-            }
-            m = block_reduce<MaxKey>(m, smem);
-            if (threadIdx.x == 0) {
-                best = m;
-                const uint32_t c = ~(uint32_t)m;
-                values[r * k + j] = x[r * cols + c];
-                indices[r * k + j] = c;
-            }
-            __syncthreads();
-            below = best;
-            __syncthreads();
+// orders the LDS accesses of the NT threads
+template <int NT>
+__device__ __forceinline__ void select_sync() {
+    if constexpr (NT == kWave) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();
+    }
+}
+
+__device__ __forceinline__ float larger(float a, float b) {  // NaN if either is
+    return __builtin_elementwise_maximum(a, b);
+}
+
+// What a value has to reach: `low` for the quick look (NaN: every value passes), `key` exactly.
+struct Bound {
+    uint32_t key;
+    float low;
+};
+
+// Four values from column col on; what lies behind the row's end is -inf, which loses to every value of the row.  ONCE: not
+// read again.
+template <bool ONCE>
+__device__ __forceinline__ float4u row_piece(const float* row, uint32_t col, uint32_t cols) {
+    if (col + 4 <= cols) {
+        const float4u* p = reinterpret_cast<const float4u*>(row + col);
+        return ONCE ? __builtin_nontemporal_load(p) : *p;
+    }
+    float4u v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (col < cols) v.x = row[col];
+    if (col + 1 < cols) v.y = row[col + 1];
+    if (col + 2 < cols) v.z = row[col + 2];
+    return v;
+}
+
+// Those of the four values that reach the bound become candidates.
+template <int NT>
+__device__ __forceinline__ void push_piece(Select<NT>& s, float4u v, uint32_t col, uint32_t cols, Bound bound) {
+    if (larger(larger(v.x, v.y), larger(v.z, v.w)) < bound.low) return;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t key = order_key(v[e]);
+        if (key < bound.key || col + e >= cols) continue;
+        const uint32_t at = atomicAdd(&s.n, 1u);
+        if (at < (uint32_t)Select<NT>::kCap) s.key[at] = element_key(key, col + e);
+    }
+}
+
+// Leaves the k largest of the s.n <= kCap candidates and returns the bound for values of later columns.  All threads call it
+// after a sync and find the candidates in place when it returns.
+template <int NT>
+__device__ Bound select_cut(Select<NT>& s, uint32_t k, int tid) {
+    const uint32_t n = s.n;
+    const int lane = tid & (kWave - 1);
+    uint64_t prefix = 0, mask = 0;
+    uint32_t need = k;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        for (int i = tid; i < 256; i += NT) s.hist[i] = 0;
+        select_sync<NT>();
+        for (uint32_t i = tid; i < n; i += NT) {
+            const uint64_t key = s.key[i];
+            if ((key & mask) == prefix) atomicAdd(&s.hist[(key >> shift) & 255], 1u);
         }
+        select_sync<NT>();
+        // every wave finds the digit: lane l looks after the digits 255 - 4l .. 252 - 4l
+        uint32_t h[4], sum = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            h[u] = s.hist[255 - 4 * lane - u];
+            sum += h[u];
+        }
+        uint32_t incl = sum;
+#pragma unroll
+        for (int d = 1; d < kWave; d <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_up((int)incl, d, kWave);
+            if (lane >= d) incl += o;
+        }
+        const int l = __builtin_ctzll(__ballot(incl >= need));
+        uint32_t above = incl - sum, digit = 0, inside = 0;
+        bool found = false;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (!found && above + h[u] >= need) {
+                found = true;
+                digit = 255 - 4 * lane - u;
+                inside = h[u];
+            }
+            if (!found) above += h[u];
+        }
+        above = (uint32_t)__builtin_amdgcn_readlane((int)above, l);
+        digit = (uint32_t)__builtin_amdgcn_readlane((int)digit, l);
+        inside = (uint32_t)__builtin_amdgcn_readlane((int)inside, l);
+        prefix |= (uint64_t)digit << shift;
+        mask |= (uint64_t)255 << shift;
+        need -= above;
+        select_sync<NT>();
+        if (inside == need) break;  // exactly the keys from here on up
+    }
+    // moved down in place: what is kept of a stretch lands where keys have been read already
+    if (tid == 0) s.n = 0;
+    select_sync<NT>();
+    for (uint32_t i0 = 0; i0 < n; i0 += NT) {
+        const uint64_t mine = i0 + tid < n ? s.key[i0 + tid] : 0;
+        select_sync<NT>();
+        if (mine >= prefix && mine != 0) s.key[atomicAdd(&s.n, 1u)] = mine;
+        select_sync<NT>();
+    }
+    // with the whole value told apart, later columns of the same value lose
+    const uint32_t top = (uint32_t)(prefix >> 32);
+    return {(uint32_t)mask ? top + 1 : top, key_value(top)};
+}
+
+// The row again, NT x 4 values at a time, with room made before each.
+template <int NT>
+__device__ void select_slowly(Select<NT>& s, const float* row, uint32_t cols, uint32_t k, int tid) {
+    Bound bound{0u, NAN};
+    select_sync<NT>();
+    if (tid == 0) s.n = 0;
+    select_sync<NT>();
+    for (uint32_t c0 = 0; c0 < cols; c0 += 4 * NT) {
+        if (s.n + 4 * NT > (uint32_t)Select<NT>::kCap) bound = select_cut<NT>(s, k, tid);
+        select_sync<NT>();
+        const uint32_t col = c0 + 4 * tid;
+        push_piece<NT>(s, row_piece<false>(row, col, cols), col, cols, bound);
+        select_sync<NT>();
+    }
+}
+
+// The candidates of a row, at least k of them, its k largest among them.
+template <int NT, int VPT>
+__device__ __forceinline__ void select_row(Select<NT>& s, const float* row, uint32_t cols, uint32_t k, int tid) {
+    constexpr uint32_t kTile = 4 * NT * VPT;
+    constexpr int U = 4;                    // pieces in flight per thread behind the tile
+    constexpr uint32_t kStretch = 4 * 4 * NT * U;  // columns between two looks at the number of candidates
+    const int lane = tid & (kWave - 1), wave = tid / kWave;
+    float4u v[VPT];
+#pragma unroll
+    for (int u = 0; u < VPT; u++) v[u] = row_piece<false>(row, 4 * (tid + u * NT), cols);
+    float4u top = v[0];  // groups: the same component of a thread's pieces
+#pragma unroll
+    for (int u = 1; u < VPT; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) top[e] = larger(top[e], v[u][e]);
+    uint32_t group[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) group[e] = order_key(top[e]);
+    if (tid == 0) s.n = 0;
+    uint32_t t = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 16; bit--) {
+        const uint32_t c = t | (1u << bit);
+        uint32_t reach = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) reach += (uint32_t)__popcll(__ballot(group[e] >= c));
+        if constexpr (NT != kWave) {
+            if (lane == 0) s.count[bit & 1][wave] = reach;
+            __syncthreads();
+            reach = 0;
+#pragma unroll
+            for (int w = 0; w < Select<NT>::kWaves; w++) reach += s.count[bit & 1][w];
+        }
+        if (reach >= k) t = c;
+    }
+    Bound bound{t, key_value(t)};
+    select_sync<NT>();
+    // a thread whose maximum reaches the bound reads its values again (from the caches): holding them costs the registers
+    // of half the waves
+    if (!(larger(larger(top[0], top[1]), larger(top[2], top[3])) < bound.low)) {
+#pragma unroll 2
+        for (uint32_t col = 4 * tid; col < kTile && col < cols; col += 4 * NT)
+            push_piece<NT>(s, row_piece<false>(row, col, cols), col, cols, bound);
+    }
+    select_sync<NT>();
+    for (uint32_t c0 = kTile; c0 < cols && s.n <= (uint32_t)Select<NT>::kCap;) {
+        if (s.n > (uint32_t)Select<NT>::kCap / 2) {
+            const Bound b = select_cut<NT>(s, k, tid);
+            if (b.key > bound.key) bound = b;
+        }
+        select_sync<NT>();
+        const uint32_t end = cols - c0 < kStretch ? cols : c0 + kStretch;
+        for (; c0 < end; c0 += 4 * NT * U) {
+            float4u w[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) w[u] = row_piece<true>(row, c0 + 4 * (tid + u * NT), cols);
+#pragma unroll
+            for (int u = 0; u < U; u++) push_piece<NT>(s, w[u], c0 + 4 * (tid + u * NT), cols, bound);
+        }
+        select_sync<NT>();
+    }
+    if (s.n > (uint32_t)Select<NT>::kCap) select_slowly<NT>(s, row, cols, k, tid);
+}
+
+// The k largest candidates in order, by rank: emit(rank, key).
+template <int NT, class Emit>
+__device__ __forceinline__ void select_emit(Select<NT>& s, uint32_t k, int tid, Emit emit) {
+    if (s.n > Select<NT>::kRankMost && s.n > k) select_cut<NT>(s, k, tid);
+    const uint32_t n = s.n;
+    if (tid < 2) s.key[n + tid] = 0;
+    select_sync<NT>();
+    for (uint32_t i = tid; i < n; i += NT) {
+        const uint64_t mine = s.key[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n; j += 2) rank += (uint32_t)(s.key[j] > mine) + (uint32_t)(s.key[j + 1] > mine);
+        if (rank < k) emit(rank, mine);
+    }
+}
+
+template <int NT, int VPT>
+__global__ __launch_bounds__(256, 4) void topk_kernel(const float* x, float* values, uint64_t* indices, size_t rows, uint32_t cols,
+                                                   uint32_t k) {
+    constexpr int kRows = 256 / NT;
+    __shared__ Select<NT> mem[kRows];
+    const int tid = threadIdx.x % NT, sub = threadIdx.x / NT;
+    Select<NT>& s = mem[sub];
+    for (size_t r = (size_t)blockIdx.x * kRows + sub; r < rows; r += (size_t)gridDim.x * kRows) {
+        const float* row = x + r * cols;
+        select_row<NT, VPT>(s, row, cols, k, tid);
+        select_emit<NT>(s, k, tid, [&](uint32_t rank, uint64_t key) {
+            const uint32_t c = ~(uint32_t)key;
+            values[r * k + rank] = row[c];
+            indices[r * k + rank] = c;
+        });
+        select_sync<NT>();
     }
 }
 
 // A row's chosen places in LDS: entry j holds its column (kNoCol: none), and only the first of the entries that name a
 // column speaks for it.
 constexpr uint32_t kNoCol = 0xffffffffu;
-constexpr int kMaxK = ZG_HIP_TOPK_MAX_K;
 __device__ __forceinline__ bool speaks(const uint32_t* col, int j) {
     const uint32_t c = col[j];
     if (c == kNoCol) return false;
@@ -227,7 +455,7 @@ static int distill_check(const char* op, const float* logits, const float* teach
                          const float* row_weights, size_t rows, size_t cols, size_t k, float temperature) {
     ZG_REQUIRE(logits && teacher && indices, "%s: null pointer", op);
     ZG_REQUIRE(((uintptr_t)indices & 7u) == 0, "%s: indices are not on an 8-byte boundary", op);
-    ZG_REQUIRE(cols < 0xffffffffull, "%s: %zu columns", op, cols);
+    ZG_REQUIRE(cols < ((size_t)1 << 31), "%s: %zu columns", op, cols);
     ZG_REQUIRE(mul_sat(rows, cols) < ((size_t)1 << 60) && mul_sat(rows, k) < ((size_t)1 << 60), "%s: %zu rows", op, rows);
     ZG_REQUIRE(k >= 1 && k <= kMaxK, "%s: k = %zu is not in 1 .. %d", op, k, kMaxK);
     ZG_REQUIRE(temperature > 0.f && temperature < INFINITY && 1.f / temperature < INFINITY, "%s: temperature %g", op, temperature);
@@ -256,7 +484,7 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
                            size_t k) {
     ZG_CTX(ctx);
     ZG_REQUIRE(k >= 1 && k <= cols && k <= kMaxK, "topk_fwd: k = %zu is not in 1 .. min(%zu, %d)", k, cols, kMaxK);
-    ZG_REQUIRE(cols < 0xffffffffull, "topk_fwd: %zu columns", cols);
+    ZG_REQUIRE(cols < ((size_t)1 << 31), "topk_fwd: %zu columns", cols);
     if (rows == 0) return ZG_HIP_OK;
     ZG_REQUIRE(x && values && indices, "topk_fwd: null pointer");
     ZG_REQUIRE(((uintptr_t)indices & 7u) == 0, "topk_fwd: indices are not on an 8-byte boundary");
@@ -265,7 +493,22 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
                    !ranges_overlap(indices, rows * k * 8, values, rows * k * 4),
                "topk_fwd: an output overlaps another operand");
     DeviceGuard guard(ctx);
-    hipLaunchKernelGGL(topk_rounds_kernel, dim3(row_grid(rows)), dim3(kBlock), 0, ctx->stream, x, values, indices, rows, cols, k);
+    const uint32_t c32 = (uint32_t)cols, k32 = (uint32_t)k;
+#define ZG_TOPK(NT, VPT)                                                                                                      \
+    hipLaunchKernelGGL((topk_kernel<NT, VPT>), dim3(row_grid(ceil_div_sz(rows, 256 / (NT)))), dim3(256), 0, ctx->stream, x, values, \
+                       indices, rows, c32, k32)
+    // A wave per row up to 2048 columns, as far as its 256 groups can bound k; a workgroup per row beyond.
+    if (cols <= 2048 && k <= 128) {
+        if (cols <= 256) ZG_TOPK(64, 1);
+        else if (cols <= 512) ZG_TOPK(64, 2);
+        else if (cols <= 1024) ZG_TOPK(64, 4);
+        else ZG_TOPK(64, 8);
+    } else if (cols <= 2048) {
+        ZG_TOPK(256, 2);
+    } else {
+        ZG_TOPK(256, 8);
+    }
+#undef ZG_TOPK
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
 }
@@ -274,7 +517,7 @@ ZG_API int zg_hip_topk_bwd(zg_hip_ctx* ctx, const uint64_t* indices, const float
                            size_t k, int accumulate) {
     ZG_CTX(ctx);
     ZG_REQUIRE(k >= 1 && k <= kMaxK, "topk_bwd: k = %zu is not in 1 .. %d", k, kMaxK);
-    ZG_REQUIRE(cols < 0xffffffffull, "topk_bwd: %zu columns", cols);
+    ZG_REQUIRE(cols < ((size_t)1 << 31), "topk_bwd: %zu columns", cols);
     if (rows == 0 || cols == 0) return ZG_HIP_OK;
     ZG_REQUIRE(indices && y_g && x_g, "topk_bwd: null pointer");
     ZG_REQUIRE(((uintptr_t)indices & 7u) == 0, "topk_bwd: indices are not on an 8-byte boundary");
