@@ -102,6 +102,36 @@ def test_many_rows(hip, rows, cols, k):
     assert np.array_equal(values, np.take_along_axis(x, want, axis=1))
 
 
+@pytest.mark.parametrize("cols", [2049, 4100, 9003])
+@pytest.mark.parametrize("k", [1, 40, 128])
+def test_many_long_rows_of_every_kind(hip, cols, k):
+    """Rows enough for the variant that gives a wave a row: eight kinds of row, each many times, in a mixed order."""
+    r = np.random.default_rng(cols + k)
+    kinds = [r.standard_normal(cols), np.arange(cols), -np.arange(cols), np.zeros(cols), r.integers(0, 5, cols),
+             np.where(r.random(cols) < 0.5, np.inf, -np.inf), np.where(r.random(cols) < 0.01, np.nan, r.standard_normal(cols)),
+             np.where(np.arange(cols) % 64 == 5, 1e3 + np.arange(cols), r.standard_normal(cols))]
+    kinds = np.stack(kinds).astype(np.float32)
+    which = r.integers(0, len(kinds), 4200)
+    values, indices = run_fwd(hip, kinds[which], k)
+    want_v, want_i = topk(kinds, k)
+    assert np.array_equal(indices, want_i[which])
+    assert np.array_equal(values, want_v[which], equal_nan=True)
+
+
+@pytest.mark.parametrize("cols", [1, 4, 5, 16, 17, 60, 64, 100, 128, 131, 256])
+def test_short_rows_of_every_kind(hip, cols):
+    r = np.random.default_rng(cols)
+    x = r.standard_normal((300, cols)).astype(np.float32)
+    x[::3] = r.integers(-1, 2, (100, cols)) * np.float32(-0.0 if cols % 2 else 1.0)
+    x[1::7, r.random(cols) < 0.3] = np.nan
+    x[2::5, r.random(cols) < 0.5] = -np.inf
+    for k in sorted({1, min(cols, 2), min(cols, 9), min(cols, 16), min(cols, 17), cols}):
+        values, indices = run_fwd(hip, x, k)
+        want_v, want_i = topk(x, k)
+        assert np.array_equal(indices, want_i)
+        assert np.array_equal(values, want_v, equal_nan=True)
+
+
 @pytest.mark.parametrize("shift", [1, 2, 3])
 def test_rows_off_the_16_byte_grid(hip, shift):
     r = np.random.default_rng(shift)

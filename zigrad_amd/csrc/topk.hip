@@ -1,6 +1,8 @@
 // The k largest of a row, and the loss of a student against a teacher's k largest logits.
 #include "reduce_device.h"
 
+#include <type_traits>
+
 namespace zg {
 
 // A float as an unsigned number of the same order: -0 like +0, every NaN above +inf.
@@ -22,30 +24,33 @@ constexpr int kMaxK = ZG_HIP_TOPK_MAX_K;
 
 // ------------------------------------------------------------------------------------------------
 // Selection.  NT threads (a wave, or a workgroup of four) own a row and read it once:
-//   * the first NT x 4 x VPT values are held in registers as 4 NT groups, and the k-th largest of the groups' maxima is a
-//     lower bound of the row's k-th largest value (k groups hold a value at least that large each).  It is found bit by
+//   * the first NT x 4 x VPT values are held in registers as groups, and the k-th largest of the groups' maxima is a lower
+//     bound of the row's k-th largest value (k groups hold a value at least that large each).  It is found bit by
 //     bit from the top, counting with ballots, and only to 16 bits: a bound that is a little low lets a few more through;
 //   * values that reach the bound become candidates in LDS as 64-bit keys (value, then column), about k of them among the
-//     first values and k / (4 NT VPT) of the rest of the row.  A thread looks at its single values only when their maximum
-//     reaches the bound, so the row is read at the memory's rate;
+//     first values and k / (4 NT VPT) of the rest of the row.  Each wave has a stretch of LDS and a counter in registers
+//     for its own, so that a candidate costs a ballot and a store (a shared LDS counter, whose answer every store had to
+//     wait for, took 332 us for 64 of 32000 in 8192 rows where this takes 202 us, 5.2 TB/s);
 //   * with more than kRankMost candidates the k largest are cut out by a radix selection over their keys (eight bits at a
 //     time, as many digits as it takes to tell them apart), which also raises the bound for the rest of the row;
 //   * a candidate's place in the result is the number of larger keys, which every thread counts for its own candidates.
 // Keys are unique, so neither the order in which candidates arrive nor the variant taken changes the result.
-// When a stretch of the row brings more candidates than LDS has room for (rows in rising order, rows of few different values) the
-// row is read again in pieces that fit whatever they hold (select_slowly).
+// When a stretch of the row brings more candidates than LDS has room for (rows in rising order, rows of few different values)
+// the row is read again in pieces that fit whatever they hold (select_slowly).
 // ------------------------------------------------------------------------------------------------
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes at any 4-byte alignment
+
+constexpr uint32_t kSegment = 1024;  // candidates a wave has room for
+constexpr uint32_t kRankMost = 384;
+constexpr int kThin = 6;             // times 64: candidates of a wave that are thinned out with ballots
 
 template <int NT>
 struct Select {
     static constexpr int kWaves = NT / kWave;
-    static constexpr int kCap = NT == kWave ? 1024 : 4096;
-    static constexpr uint32_t kRankMost = 384;
-    uint64_t key[kCap + 2];
+    uint64_t key[kWaves][kSegment + 2];
     uint32_t hist[256];
-    uint32_t count[2][kWaves];
-    uint32_t n;  // candidates asked for; those past kCap found no room
+    uint32_t low[kWaves];       // the waves' bounds
+    uint32_t n[kWaves];         // candidates, written down where other waves need them
 };
 
 // orders the LDS accesses of the NT threads
@@ -63,53 +68,101 @@ __device__ __forceinline__ float larger(float a, float b) {  // NaN if either is
     return __builtin_elementwise_maximum(a, b);
 }
 
-// What a value has to reach: `low` for the quick look (NaN: every value passes), `key` exactly.
+// What a value has to reach, as a key and as that key's number (NaN where there is none: every value passes).
 struct Bound {
     uint32_t key;
     float low;
 };
+__device__ __forceinline__ Bound bound_of(uint32_t key) { return {key, key_value(key)}; }
 
-// Four values from column col on; what lies behind the row's end is -inf, which loses to every value of the row.  ONCE: not
-// read again.
-template <bool ONCE>
-__device__ __forceinline__ float4u row_piece(const float* row, uint32_t col, uint32_t cols) {
-    if (col + 4 <= cols) {
-        const float4u* p = reinterpret_cast<const float4u*>(row + col);
-        return ONCE ? __builtin_nontemporal_load(p) : *p;
-    }
-    float4u v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    if (col < cols) v.x = row[col];
-    if (col + 1 < cols) v.y = row[col + 1];
-    if (col + 2 < cols) v.z = row[col + 2];
-    return v;
+// The thread's place: its number among the NT, its wave, its lane; n: the wave's candidates, the same in all its lanes, of which
+// the first `keyed` are in LDS as keys and the rest as they came, (bits of the value, column).
+struct Place {
+    int tid, wave, lane;
+    uint32_t n, keyed;
+};
+
+// Whole pieces of four values of a row, from `base` (the same in all lanes) on; `bytes`: how far the row's whole pieces reach from
+// there.  Pieces behind that are -inf, which loses to every value of the row: a buffer load takes any 4-byte alignment and
+// reads nothing behind the end.
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ float4u row_piece(const float* base, uint32_t bytes, uint32_t off) {
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, (int)bytes, 0x00020000);
+    const float4u v = __builtin_bit_cast(float4u, (uint4v)__builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, 0));
+    const bool in = off < bytes;
+    return float4u{in ? v.x : -INFINITY, in ? v.y : -INFINITY, in ? v.z : -INFINITY, in ? v.w : -INFINITY};
+}
+__device__ __forceinline__ uint32_t bytes_from(uint32_t c0, uint32_t whole) {  // whole: columns in whole pieces
+    const uint32_t left = c0 < whole ? whole - c0 : 0u;
+    return left < (1u << 28) ? left * 4u : 1u << 30;
+}
+__device__ __forceinline__ uint32_t lanes_below(uint64_t lanes) {  // how many of `lanes` are below this one
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u));
 }
 
-// Those of the four values that reach the bound become candidates.
-template <int NT>
-__device__ __forceinline__ void push_piece(Select<NT>& s, float4u v, uint32_t col, uint32_t cols, Bound bound) {
-    if (larger(larger(v.x, v.y), larger(v.z, v.w)) < bound.low) return;
+// Those of the four values that reach the bound become candidates of the wave, all of whose lanes call this.  Candidates past
+// kSegment are counted and find no room.  CHECK: columns from `cols` on are none.
+template <int NT, bool CHECK>
+__device__ __forceinline__ void push_piece(Select<NT>& s, Place& at, float4u v, uint32_t col, uint32_t cols, float low) {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        const uint32_t key = order_key(v[e]);
-        if (key < bound.key || col + e >= cols) continue;
-        const uint32_t at = atomicAdd(&s.n, 1u);
-        if (at < (uint32_t)Select<NT>::kCap) s.key[at] = element_key(key, col + e);
+        const bool in = !(v[e] < low) && (!CHECK || col + e < cols);
+        const uint64_t ins = __ballot(in);
+        if (!ins) continue;
+        const uint32_t to = at.n + lanes_below(ins);
+        if (in && to < kSegment) s.key[at.wave][to] = ((uint64_t)__float_as_uint(v[e]) << 32) | (col + e);
+        at.n += (uint32_t)__popcll(ins);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // a piece at a time: done side by side they cost the registers of half the waves
+}
+// The up to three values behind the row's whole pieces.
+template <int NT>
+__device__ __forceinline__ void push_tail(Select<NT>& s, Place& at, const float* row, uint32_t whole, uint32_t cols, float low) {
+    if (whole == cols || at.wave != 0) return;
+    const uint32_t col = whole + at.lane;
+    const float x = col < cols ? row[col] : -INFINITY;
+    push_piece<NT, true>(s, at, float4u{x, -INFINITY, -INFINITY, -INFINITY}, col, col < cols ? col + 1 : 0u, low);
+}
+// The candidates that came since are turned into keys.
+template <int NT>
+__device__ __forceinline__ void key_candidates(Select<NT>& s, Place& at) {
+    select_sync<kWave>();
+    for (uint32_t i = at.keyed + at.lane; i < at.n; i += kWave) {
+        const uint64_t c = s.key[at.wave][i];
+        s.key[at.wave][i] = element_key(order_key(__uint_as_float((uint32_t)(c >> 32))), (uint32_t)c);
+    }
+    at.keyed = at.n;
+}
+
+// The most candidates any wave has; a sync.
+template <int NT>
+__device__ __forceinline__ uint32_t select_most(Select<NT>& s, const Place& at) {
+    if constexpr (NT == kWave) {
+        select_sync<NT>();
+        return at.n;
+    } else {
+        if (at.lane == 0) s.n[at.wave] = at.n;
+        __syncthreads();
+        uint32_t most = 0;
+#pragma unroll
+        for (int w = 0; w < Select<NT>::kWaves; w++) most = s.n[w] > most ? s.n[w] : most;
+        return most;
     }
 }
 
-// Leaves the k largest of the s.n <= kCap candidates and returns the bound for values of later columns.  All threads call it
-// after a sync and find the candidates in place when it returns.
+// Leaves the k largest of the candidates (none lost, at least k) and returns the bound for values of later columns.  All threads
+// call it after select_most.
 template <int NT>
-__device__ Bound select_cut(Select<NT>& s, uint32_t k, int tid) {
-    const uint32_t n = s.n;
-    const int lane = tid & (kWave - 1);
+__device__ Bound select_cut(Select<NT>& s, Place& at, uint32_t k) {
+    const int lane = at.lane;
+    key_candidates<NT>(s, at);
     uint64_t prefix = 0, mask = 0;
     uint32_t need = k;
     for (int shift = 56; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += NT) s.hist[i] = 0;
+        for (int i = at.tid; i < 256; i += NT) s.hist[i] = 0;
         select_sync<NT>();
-        for (uint32_t i = tid; i < n; i += NT) {
-            const uint64_t key = s.key[i];
+        for (uint32_t i = lane; i < at.n; i += kWave) {
+            const uint64_t key = s.key[at.wave][i];
             if ((key & mask) == prefix) atomicAdd(&s.hist[(key >> shift) & 255], 1u);
         }
         select_sync<NT>();
@@ -147,47 +200,119 @@ __device__ Bound select_cut(Select<NT>& s, uint32_t k, int tid) {
         select_sync<NT>();
         if (inside == need) break;  // exactly the keys from here on up
     }
-    // moved down in place: what is kept of a stretch lands where keys have been read already
-    if (tid == 0) s.n = 0;
-    select_sync<NT>();
-    for (uint32_t i0 = 0; i0 < n; i0 += NT) {
-        const uint64_t mine = i0 + tid < n ? s.key[i0 + tid] : 0;
-        select_sync<NT>();
-        if (mine >= prefix && mine != 0) s.key[atomicAdd(&s.n, 1u)] = mine;
-        select_sync<NT>();
+    // each wave moves its own down: what is kept lands where keys have been read already
+    uint32_t kept = 0;
+    for (uint32_t i0 = 0; i0 < at.n; i0 += kWave) {
+        const uint64_t mine = i0 + lane < at.n ? s.key[at.wave][i0 + lane] : 0;
+        const bool in = mine >= prefix && mine != 0;
+        const uint64_t ins = __ballot(in);
+        select_sync<kWave>();
+        if (in) s.key[at.wave][kept + lanes_below(ins)] = mine;
+        select_sync<kWave>();
+        kept += (uint32_t)__popcll(ins);
     }
+    at.n = at.keyed = kept;
     // with the whole value told apart, later columns of the same value lose
     const uint32_t top = (uint32_t)(prefix >> 32);
-    return {(uint32_t)mask ? top + 1 : top, key_value(top)};
+    return bound_of((uint32_t)mask ? top + 1 : top);
+}
+
+// The largest number t of 16 bits, then zeros, that at least `share` of the wave's keys reach; 0 when it has fewer.  KEYS keys a lane.
+template <int KEYS>
+__device__ __forceinline__ uint32_t wave_bound(const uint32_t (&key)[KEYS], uint32_t share) {
+    uint32_t t = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 16; bit--) {
+        const uint32_t c = t | (1u << bit);
+        uint32_t reach = 0;
+#pragma unroll
+        for (int e = 0; e < KEYS; e++) reach += (uint32_t)__popcll(__ballot(key[e] >= c));
+        if (reach >= share) t = c;
+        if (reach == share) break;  // no need to know the bound better
+    }
+    return t;
+}
+// The lowest of the waves' bounds: k values of the row reach it when each wave bounds its share of k.
+template <int NT>
+__device__ __forceinline__ uint32_t lowest_bound(Select<NT>& s, const Place& at, uint32_t t) {
+    if constexpr (NT != kWave) {
+        if (at.lane == 0) s.low[at.wave] = t;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < Select<NT>::kWaves; w++) t = s.low[w] < t ? s.low[w] : t;
+    }
+    return t;
+}
+
+// Drops candidates that a bound from the candidates themselves excludes (a few hundred come down to little more than k; ranking is
+// quadratic in what is left) and returns that bound.  No wave has more than 64 KEYS; all threads call it after a sync.
+template <int NT, int KEYS>
+__device__ __forceinline__ uint32_t select_thin(Select<NT>& s, Place& at, uint32_t share) {
+    key_candidates<NT>(s, at);
+    select_sync<kWave>();
+    uint32_t key[KEYS];
+#pragma unroll
+    for (int e = 0; e < KEYS; e++) {
+        const uint32_t i = at.lane + e * kWave;
+        key[e] = i < at.n ? (uint32_t)(s.key[at.wave][i] >> 32) : 0u;
+    }
+    const uint32_t t = lowest_bound<NT>(s, at, wave_bound<KEYS>(key, share));
+    uint32_t kept = 0;
+#pragma unroll
+    for (int e = 0; e < KEYS; e++) {
+        const uint32_t i = at.lane + e * kWave;
+        const bool in = i < at.n && key[e] >= t;
+        const uint64_t ins = __ballot(in);
+        if (!ins) continue;
+        const uint32_t low = (uint32_t)s.key[at.wave][i < at.n ? i : 0];
+        select_sync<kWave>();
+        if (in) s.key[at.wave][kept + lanes_below(ins)] = ((uint64_t)key[e] << 32) | low;
+        select_sync<kWave>();
+        kept += (uint32_t)__popcll(ins);
+    }
+    at.n = at.keyed = kept;
+    return t;
 }
 
 // The row again, NT x 4 values at a time, with room made before each.
 template <int NT>
-__device__ void select_slowly(Select<NT>& s, const float* row, uint32_t cols, uint32_t k, int tid) {
-    Bound bound{0u, NAN};
-    select_sync<NT>();
-    if (tid == 0) s.n = 0;
-    select_sync<NT>();
-    for (uint32_t c0 = 0; c0 < cols; c0 += 4 * NT) {
-        if (s.n + 4 * NT > (uint32_t)Select<NT>::kCap) bound = select_cut<NT>(s, k, tid);
-        select_sync<NT>();
-        const uint32_t col = c0 + 4 * tid;
-        push_piece<NT>(s, row_piece<false>(row, col, cols), col, cols, bound);
+__device__ void select_slowly(Select<NT>& s, Place& at, const float* row, uint32_t cols, uint32_t k) {
+    const uint32_t whole = cols & ~3u;
+    Bound bound = bound_of(0u);
+    at.n = at.keyed = 0;
+    for (uint32_t c0 = 0; c0 < cols; c0 += 4 * NT) {  // (the last round may hold nothing but the tail)
+        if (select_most<NT>(s, at) > kSegment - 5 * kWave) bound = select_cut<NT>(s, at, k);
+        push_piece<NT, true>(s, at, row_piece(row + c0, bytes_from(c0, whole), 16 * at.tid), c0 + 4 * at.tid, whole, bound.low);
+        if (cols - c0 <= 4 * NT) push_tail<NT>(s, at, row, whole, cols, bound.low);
         select_sync<NT>();
     }
 }
 
 // The candidates of a row, at least k of them, its k largest among them.
-template <int NT, int VPT>
-__device__ __forceinline__ void select_row(Select<NT>& s, const float* row, uint32_t cols, uint32_t k, int tid) {
-    constexpr uint32_t kTile = 4 * NT * VPT;
-    constexpr int U = 4;                    // pieces in flight per thread behind the tile
-    constexpr uint32_t kStretch = 4 * 4 * NT * U;  // columns between two looks at the number of candidates
-    const int lane = tid & (kWave - 1), wave = tid / kWave;
-    float4u v[VPT];
+// BEYOND: rows may be longer than the tile.
+// v: the row's tile (load_tile); `next` (null: none): the row whose tile takes its place while this row's candidates are sorted out.
+template <int NT, int VPT, bool BEYOND>
+__device__ __forceinline__ void load_tile(float4u (&v)[VPT], const Place& at, const float* row, uint32_t cols) {
 #pragma unroll
-    for (int u = 0; u < VPT; u++) v[u] = row_piece<false>(row, 4 * (tid + u * NT), cols);
-    float4u top = v[0];  // groups: the same component of a thread's pieces
+    for (int u = 0; u < VPT; u++)
+        v[u] = BEYOND ? __builtin_nontemporal_load(reinterpret_cast<const float4u*>(row) + at.tid + u * NT)
+                      : row_piece(row, bytes_from(0, cols & ~3u), 16 * (at.tid + u * NT));
+}
+template <int NT, int VPT, bool BEYOND>
+__device__ __forceinline__ void select_row(Select<NT>& s, Place& at, float4u (&v)[VPT], const float* row, const float* next,
+                                           uint32_t cols, uint32_t k) {
+    constexpr uint32_t kTile = 4 * NT * VPT;
+    constexpr int U = 4;                    // pieces in flight per thread behind the tile, twice
+    constexpr uint32_t kStep = 4 * NT * U;  // their columns
+    const uint32_t whole = cols & ~3u;
+    // behind the tile a step of pieces is looked through while the next one is on its way
+    float4u w[2][U];
+    auto load = [&](float4u (&to)[U], uint32_t c0) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            to[u] = __builtin_nontemporal_load(reinterpret_cast<const float4u*>(row + c0) + at.tid + u * NT);
+    };
+    float4u top = v[0];
 #pragma unroll
     for (int u = 1; u < VPT; u++)
 #pragma unroll
@@ -195,83 +320,272 @@ __device__ __forceinline__ void select_row(Select<NT>& s, const float* row, uint
     uint32_t group[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) group[e] = order_key(top[e]);
-    if (tid == 0) s.n = 0;
-    uint32_t t = 0;
-#pragma unroll 1
-    for (int bit = 31; bit >= 16; bit--) {
-        const uint32_t c = t | (1u << bit);
-        uint32_t reach = 0;
+    // each wave bounds its share of k by its own groups, without waiting for the others
+    const uint32_t share = (k + Select<NT>::kWaves - 1) / Select<NT>::kWaves;
+    Bound bound = bound_of(lowest_bound<NT>(s, at, wave_bound<4>(group, share)));
+    at.n = at.keyed = 0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) reach += (uint32_t)__popcll(__ballot(group[e] >= c));
-        if constexpr (NT != kWave) {
-            if (lane == 0) s.count[bit & 1][wave] = reach;
-            __syncthreads();
-            reach = 0;
+    for (int u = 0; u < VPT; u++) push_piece<NT, !BEYOND>(s, at, v[u], 4 * (at.tid + u * NT), whole, bound.low);
+    push_tail<NT>(s, at, row, whole, cols, bound.low);
+    if constexpr (BEYOND) {
+        bool room = true;
+        uint32_t c0 = kTile;
+        // A look at the number of candidates: a wave by itself raises its bound whenever they are twice k, a workgroup, whose waves
+        // have to meet for it, every four steps when LDS fills up.
+        auto look = [&]() {
+            if constexpr (NT == kWave) {
+                if (at.n <= 2 * k + kWave) return;
+                room = at.n <= kSegment;
+                if (!room) return;
+                Bound b;
+                if (at.n <= kThin * kWave) b = bound_of(select_thin<NT, kThin>(s, at, k));
+                else b = select_cut<NT>(s, at, k);
+                if (b.key > bound.key) bound = b;
+            } else if ((c0 - kTile) % (4 * kStep) == 0) {
+                const uint32_t most = select_most<NT>(s, at);
+                room = most <= kSegment;
+                if (!room) return;
+                if (most > kSegment / 2) {
+                    const Bound b = select_cut<NT>(s, at, k);
+                    if (b.key > bound.key) bound = b;
+                }
+                select_sync<NT>();
+            }
+        };
+        if (kTile + kStep <= whole) load(w[0], kTile);
+        while (c0 + kStep <= whole) {
+            look();
+            if (!room) break;
+            const bool more = c0 + 2 * kStep <= whole;
+            if (more) load(w[1], c0 + kStep);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int w = 0; w < Select<NT>::kWaves; w++) reach += s.count[bit & 1][w];
+            for (int u = 0; u < U; u++) push_piece<NT, false>(s, at, w[0][u], c0 + 4 * (at.tid + u * NT), whole, bound.low);
+            c0 += kStep;
+            if (!more) break;
+            if constexpr (NT == kWave) {
+                look();
+                if (!room) break;
+            }
+            if (c0 + 2 * kStep <= whole) load(w[0], c0 + kStep);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < U; u++) push_piece<NT, false>(s, at, w[1][u], c0 + 4 * (at.tid + u * NT), whole, bound.low);
+            c0 += kStep;
         }
-        if (reach >= k) t = c;
-    }
-    Bound bound{t, key_value(t)};
-    select_sync<NT>();
-    // a thread whose maximum reaches the bound reads its values again (from the caches): holding them costs the registers
-    // of half the waves
-    if (!(larger(larger(top[0], top[1]), larger(top[2], top[3])) < bound.low)) {
-#pragma unroll 2
-        for (uint32_t col = 4 * tid; col < kTile && col < cols; col += 4 * NT)
-            push_piece<NT>(s, row_piece<false>(row, col, cols), col, cols, bound);
-    }
-    select_sync<NT>();
-    for (uint32_t c0 = kTile; c0 < cols && s.n <= (uint32_t)Select<NT>::kCap;) {
-        if (s.n > (uint32_t)Select<NT>::kCap / 2) {
-            const Bound b = select_cut<NT>(s, k, tid);
-            if (b.key > bound.key) bound = b;
+        if (room && c0 < whole) {  // less than a step
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                push_piece<NT, true>(s, at, row_piece(row + c0, bytes_from(c0, whole), 16 * (at.tid + u * NT)), c0 + 4 * (at.tid + u * NT),
+                                     whole, bound.low);
         }
+    }
+    if (next) load_tile<NT, VPT, BEYOND>(v, at, next, cols);
+    if (select_most<NT>(s, at) > kSegment) {
         select_sync<NT>();
-        const uint32_t end = cols - c0 < kStretch ? cols : c0 + kStretch;
-        for (; c0 < end; c0 += 4 * NT * U) {
-            float4u w[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) w[u] = row_piece<true>(row, c0 + 4 * (tid + u * NT), cols);
-#pragma unroll
-            for (int u = 0; u < U; u++) push_piece<NT>(s, w[u], c0 + 4 * (tid + u * NT), cols, bound);
-        }
-        select_sync<NT>();
+        select_slowly<NT>(s, at, row, cols, k);
     }
-    if (s.n > (uint32_t)Select<NT>::kCap) select_slowly<NT>(s, row, cols, k, tid);
+    key_candidates<NT>(s, at);
 }
 
 // The k largest candidates in order, by rank: emit(rank, key).
 template <int NT, class Emit>
-__device__ __forceinline__ void select_emit(Select<NT>& s, uint32_t k, int tid, Emit emit) {
-    if (s.n > Select<NT>::kRankMost && s.n > k) select_cut<NT>(s, k, tid);
-    const uint32_t n = s.n;
-    if (tid < 2) s.key[n + tid] = 0;
+__device__ __forceinline__ void select_emit(Select<NT>& s, Place& at, uint32_t k, Emit emit) {
+    constexpr int kWaves = Select<NT>::kWaves;
+    uint32_t all = 0;
+    auto total = [&]() {
+        select_sync<NT>();
+        select_most<NT>(s, at);
+        all = 0;
+        if constexpr (NT == kWave) {
+            all = at.n;
+        } else {
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) all += s.n[w];
+        }
+    };
+    total();
+    if (all > k + k / 2 + 16) {
+        constexpr int kKeys = NT == kWave ? kThin : 2;
+        if (select_most<NT>(s, at) <= kKeys * kWave) {
+            select_thin<NT, kKeys>(s, at, (k + kWaves - 1) / kWaves);
+            total();
+        }
+    }
+    if (all > kRankMost && all > k) {
+        select_cut<NT>(s, at, k);
+        total();
+    }
+    if (at.lane < 2) s.key[at.wave][at.n + at.lane] = 0;
     select_sync<NT>();
-    for (uint32_t i = tid; i < n; i += NT) {
-        const uint64_t mine = s.key[i];
+    // the threads take the candidates of all waves in turn
+    for (uint32_t i = at.tid; i < all; i += NT) {
+        uint64_t mine;
+        if constexpr (NT == kWave) {
+            mine = s.key[0][i];
+        } else {
+            uint32_t j = i;
+            int w = 0;
+            while (j >= s.n[w]) j -= s.n[w++];
+            mine = s.key[w][j];
+        }
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; j += 2) rank += (uint32_t)(s.key[j] > mine) + (uint32_t)(s.key[j + 1] > mine);
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const uint32_t n = NT == kWave ? at.n : s.n[w];
+#pragma unroll 8
+            for (uint32_t j = 0; j < n; j += 2) rank += (uint32_t)(s.key[w][j] > mine) + (uint32_t)(s.key[w][j + 1] > mine);
+        }
         if (rank < k) emit(rank, mine);
     }
 }
 
-template <int NT, int VPT>
+template <int NT, int VPT, bool BEYOND>
 __global__ __launch_bounds__(256, 4) void topk_kernel(const float* x, float* values, uint64_t* indices, size_t rows, uint32_t cols,
-                                                   uint32_t k) {
+                                                      uint32_t k) {
     constexpr int kRows = 256 / NT;
     __shared__ Select<NT> mem[kRows];
-    const int tid = threadIdx.x % NT, sub = threadIdx.x / NT;
+    const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));  // scalars: the row and its pieces' base are then too
+    Place at{(int)(threadIdx.x % NT), NT == kWave ? 0 : w, (int)(threadIdx.x % kWave), 0u, 0u};
+    const int sub = NT == kWave ? w : 0;
     Select<NT>& s = mem[sub];
-    for (size_t r = (size_t)blockIdx.x * kRows + sub; r < rows; r += (size_t)gridDim.x * kRows) {
+    const size_t step = (size_t)gridDim.x * kRows;
+    size_t r = (size_t)blockIdx.x * kRows + sub;
+    if (r >= rows) return;  // (only waves that own a row of their own: no barrier is missed)
+    float4u v[VPT];
+    load_tile<NT, VPT, BEYOND>(v, at, x + r * cols, cols);
+    for (; r < rows; r += step) {
         const float* row = x + r * cols;
-        select_row<NT, VPT>(s, row, cols, k, tid);
-        select_emit<NT>(s, k, tid, [&](uint32_t rank, uint64_t key) {
+        select_row<NT, VPT, BEYOND>(s, at, v, row, r + step < rows ? x + (r + step) * cols : nullptr, cols, k);
+        select_emit<NT>(s, at, k, [&](uint32_t rank, uint64_t key) {
             const uint32_t c = ~(uint32_t)key;
-            values[r * k + rank] = row[c];
+            float v = key_value((uint32_t)(key >> 32));
+            if (v == 0.f || v != v) v = row[c];  // the key knows neither the sign of a zero nor which NaN it was
+            values[r * k + rank] = v;
             indices[r * k + rank] = c;
         });
         select_sync<NT>();
+    }
+}
+
+// A few long rows: a workgroup per segment of a row leaves the segment's k largest, in order, as keys with the row's columns ...
+constexpr uint32_t kTopkSegment = 4096;
+__global__ __launch_bounds__(256, 4) void topk_segments_kernel(const float* x, uint64_t* keys, uint32_t cols, uint32_t k, uint32_t len,
+                                                               uint32_t n_seg) {
+    __shared__ Select<256> s;
+    Place at{(int)threadIdx.x, __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)), (int)(threadIdx.x % kWave), 0u, 0u};
+    const size_t r = blockIdx.x / n_seg;
+    const uint32_t seg = blockIdx.x % n_seg, c0 = seg * len, n = cols - c0 < len ? cols - c0 : len;
+    const float* part = x + r * cols + c0;
+    float4u v[4];
+    load_tile<256, 4, false>(v, at, part, n);
+    select_row<256, 4, false>(s, at, v, part, nullptr, n, k);
+    select_emit<256>(s, at, k, [&](uint32_t rank, uint64_t key) {
+        keys[((size_t)blockIdx.x) * k + rank] = (key & ~(uint64_t)0xffffffffu) | (uint32_t)~(~(uint32_t)key + c0);
+    });
+}
+// ... and a workgroup per row takes the k largest of those.  Each segment's share-th key is known, and the lowest of them is a bound.
+__global__ __launch_bounds__(256, 4) void topk_join_kernel(const float* x, const uint64_t* keys, float* values, uint64_t* indices,
+                                                           uint32_t cols, uint32_t k, uint32_t n_seg) {
+    __shared__ Select<256> s;
+    __shared__ uint64_t bounds[4];
+    Place at{(int)threadIdx.x, __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)), (int)(threadIdx.x % kWave), 0u, 0u};
+    const size_t r = blockIdx.x;
+    const uint64_t* list = keys + r * n_seg * k;
+    const uint32_t share = (k + n_seg - 1) / n_seg, total = n_seg * k;
+    uint64_t low = ~(uint64_t)0;
+    for (uint32_t i = threadIdx.x; i < n_seg; i += 256) {
+        const uint64_t b = list[(size_t)i * k + share - 1];
+        low = b < low ? b : low;
+    }
+#pragma unroll
+    for (int m = kWave / 2; m >= 1; m >>= 1) {
+        const uint64_t o = (uint64_t)__shfl_xor((unsigned long long)low, m, kWave);
+        low = o < low ? o : low;
+    }
+    if (at.lane == 0) bounds[at.wave] = low;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; w++) low = bounds[w] < low ? bounds[w] : low;
+    for (uint32_t i0 = 0; i0 < total; i0 += 256) {
+        if (i0 % (256 * 8) == 0 && i0 && select_most<256>(s, at) > kSegment - 8 * kWave) select_cut<256>(s, at, k);
+        const uint64_t key = i0 + threadIdx.x < total ? list[i0 + threadIdx.x] : 0;
+        const uint64_t ins = __ballot(key >= low && key != 0);
+        if (key >= low && key != 0) s.key[at.wave][at.n + lanes_below(ins)] = key;
+        at.n += (uint32_t)__popcll(ins);
+        at.keyed = at.n;
+        if (i0 % (256 * 8) == 0) __syncthreads();
+    }
+    select_emit<256>(s, at, k, [&](uint32_t rank, uint64_t key) {
+        const uint32_t c = ~(uint32_t)key;
+        float v = key_value((uint32_t)(key >> 32));
+        if (v == 0.f || v != v) v = x[r * cols + c];
+        values[r * k + rank] = v;
+        indices[r * k + rank] = c;
+    });
+}
+
+// Short rows and few of their values chosen (a router's scores): L lanes share a row, each holding KPL adjacent columns as keys in
+// registers, and the largest is taken out k times (8 of 128 in 65536 rows: 15 us, a wave per row with a bound and candidates 45 us).  A round is a handful of maxima across the lanes; a tie goes to the lowest lane
+// and there to the lowest column, which is the lowest column of the row.
+template <int L>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    auto step = [&](auto ctrl) {
+        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, false);
+        v = o > v ? o : v;
+    };
+    step(std::integral_constant<int, 0xB1>{});  // neighbours in pairs
+    step(std::integral_constant<int, 0x4E>{});  // pairs in quads
+    if (L == 16) {
+        step(std::integral_constant<int, 0x124>{});  // rotations of the 16 by a quad and by two
+        step(std::integral_constant<int, 0x128>{});
+    }
+    return v;
+}
+template <int L, int KPL>
+__global__ __launch_bounds__(256) void topk_short_kernel(const float* x, float* values, uint64_t* indices, size_t rows, uint32_t cols,
+                                                         uint32_t k) {
+    const size_t r = (size_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const uint32_t lane = threadIdx.x % L, first = lane * KPL;
+    const bool live = r < rows;
+    const float* row = x + (live ? r : 0) * cols;
+    uint32_t key[KPL];
+#pragma unroll
+    for (int p = 0; p < KPL; p += 4) {
+        const uint32_t c = first + p;
+        if (live && c + 4 <= cols) {
+            const float4u v = __builtin_nontemporal_load(reinterpret_cast<const float4u*>(row + c));
+#pragma unroll
+            for (int e = 0; e < 4; e++) key[p + e] = order_key(v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) key[p + e] = live && c + e < cols ? order_key(row[c + e]) : 0u;
+        }
+    }
+    for (uint32_t j = 0; j < k; j++) {
+        uint32_t mine = key[0];
+#pragma unroll
+        for (int e = 1; e < KPL; e++) mine = key[e] > mine ? key[e] : mine;
+        const uint32_t top = lanes_max<L>(mine);
+        const uint32_t shift = threadIdx.x & (kWave - 1) & ~(L - 1);
+        const uint32_t holders = (uint32_t)(__ballot(mine == top) >> shift) & ((1u << L) - 1);
+        if ((uint32_t)__builtin_ctz(holders) == lane) {
+            uint32_t at = 0;
+            bool found = false;
+#pragma unroll
+            for (int e = 0; e < KPL; e++) {
+                const bool hit = !found && key[e] == top;
+                at = hit ? (uint32_t)e : at;
+                key[e] = hit ? 0u : key[e];
+                found = found || hit;
+            }
+            if (live) {
+                float v = key_value(top);
+                if (v == 0.f || v != v) v = row[first + at];  // the key knows neither the sign of a zero nor which NaN it was
+                values[r * k + j] = v;
+                indices[r * k + j] = first + at;
+            }
+        }
     }
 }
 
@@ -286,28 +600,131 @@ __device__ __forceinline__ bool speaks(const uint32_t* col, int j) {
     return true;
 }
 
-template <bool ACC>
-__global__ __launch_bounds__(kBlock) void topk_bwd_kernel(const uint64_t* indices, const float* y_g, float* x_g, size_t rows,
-                                                           size_t cols, size_t k) {
-    __shared__ uint32_t col[kMaxK];
-    __shared__ float g[kMaxK];
-    for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        __syncthreads();
-        for (int j = threadIdx.x; j < (int)k; j += kBlock) {
-            const uint64_t c = indices[r * k + j];
-            col[j] = c < cols ? (uint32_t)c : kNoCol;
-            g[j] = y_g[r * k + j];
+// The gradient of a selection, dense, for short rows and few places: 16 lanes share a row, every lane compares its columns with each
+// chosen one (the gradients of a repeated index are added in the order of j by themselves).
+template <int P>  // pieces of four columns a lane has: 64 P columns at most
+__global__ __launch_bounds__(256) void topk_bwd_short_kernel(const uint64_t* indices, const float* y_g, float* x_g, size_t rows,
+                                                             uint32_t cols, uint32_t k) {
+    const size_t r = (size_t)blockIdx.x * 16 + threadIdx.x / 16;
+    if (r >= rows) return;
+    const uint64_t* idx = indices + r * k;
+    const float* g = y_g + r * k;
+    float* row = x_g + r * cols;
+    const uint32_t first = threadIdx.x % 16 * 4;
+    float4u v[P];
+#pragma unroll
+    for (int p = 0; p < P; p++) v[p] = float4u{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t j = 0; j < k; j++) {
+        const uint64_t c = idx[j];
+        const uint32_t at = c < cols ? (uint32_t)c - first : ~0u - 255u;  // no lane's column
+        const float a = g[j];
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[p][e] = at == (uint32_t)(64 * p + e) ? __fadd_rn(v[p][e], a) : v[p][e];
+    }
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        const uint32_t c = first + 64 * p;
+        if (c + 4 <= cols) {
+            __builtin_nontemporal_store(v[p], reinterpret_cast<float4u*>(row + c));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+                if (c + e < cols) row[c + e] = v[p][e];
         }
-        float* row = x_g + r * cols;
-        if (!ACC)
-            for (size_t c = threadIdx.x; c < cols; c += kBlock) row[c] = 0.f;
+    }
+}
+
+// The lanes of `among` that hold the same number of `bits` bits as this one.
+__device__ __forceinline__ uint64_t same_lanes(uint32_t v, int bits, uint64_t among) {
+    for (int b = 0; b < bits; b++) {
+        const bool one = (v >> b) & 1u;
+        const uint64_t ones = __ballot(one);
+        among &= one ? ones : ~ones;
+    }
+    return among;
+}
+// Adds the entries of a wave to a row, one a lane: `same`, the lanes that name this lane's column (none: no entry); the lowest of them
+// writes, the gradients in the order of the lanes.  FRESH: nothing is there yet.
+template <bool FRESH>
+__device__ __forceinline__ void add_entries(float* at, float g, uint64_t same, int lane) {
+    const bool writes = same != 0 && (same & (((uint64_t)1 << lane) - 1)) == 0;
+    float v = (!FRESH && writes) ? __fadd_rn(*at, g) : g;
+    uint64_t rest = writes ? same & (same - 1) : 0;
+    while (__any(rest != 0)) {
+        const int l = rest ? __builtin_ctzll(rest) : lane;
+        const float a = __shfl(g, l, kWave);
+        if (rest) v = __fadd_rn(v, a);
+        rest &= rest - 1;
+    }
+    if (writes) *at = v;
+}
+
+// The same for any row: a workgroup puts together kBwdSpan columns in LDS, which holds zeros but for the entries its first wave adds, 64
+// at a time, and takes out again once the span is stored.  (Clearing the span in memory and writing the entries after it, each a
+// part of a line, took 241 us for 64 of 32000 in 8192 rows, this 202 us, 5.2 TB/s.)
+constexpr uint32_t kBwdSpan = 4096;
+__device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__global__ __launch_bounds__(256) void topk_bwd_kernel(const uint64_t* indices, const float* y_g, float* x_g, size_t rows,
+                                                       uint32_t cols, uint32_t k, uint32_t spans, int bits) {
+    __shared__ __attribute__((aligned(16))) float span[kBwdSpan];
+    const int lane = threadIdx.x % kWave;
+    const bool first = threadIdx.x < kWave;
+    for (uint32_t c = threadIdx.x; c < kBwdSpan; c += 256) span[c] = 0.f;
+    const size_t jobs = rows * spans;
+    for (size_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+        const size_t r = job / spans;
+        const uint32_t c0 = (uint32_t)(job - r * spans) * kBwdSpan, n = cols - c0 < kBwdSpan ? cols - c0 : kBwdSpan;
+        float* row = x_g + r * cols + c0;
         __syncthreads();
-        for (int j = threadIdx.x; j < (int)k; j += kBlock) {
-            if (!speaks(col, j)) continue;
-            float v = ACC ? __fadd_rn(row[col[j]], g[j]) : g[j];
-            for (int i = j + 1; i < (int)k; i++)
-                if (col[i] == col[j]) v = __fadd_rn(v, g[i]);
-            row[col[j]] = v;
+        if (first) {
+            for (uint32_t j0 = 0; j0 < k; j0 += kWave) {
+                const uint64_t at = (j0 + lane < k ? indices[r * k + j0 + lane] : ~(uint64_t)0) - c0;
+                const bool here = at < n;
+                const uint64_t heres = __ballot(here);
+                if (!heres) continue;
+                const uint32_t col = here ? (uint32_t)at : 0u;
+                const float g = here ? y_g[r * k + j0 + lane] : 0.f;
+                uint64_t same = same_lanes(col, bits, heres);
+                if (!here) same = 0;
+                add_entries<false>(span + col, g, same, lane);
+                select_sync<kWave>();
+            }
+        }
+        __syncthreads();
+        uint32_t c = 4 * threadIdx.x;
+        for (; c + 4 <= n; c += 4 * 256)
+            __builtin_nontemporal_store(*reinterpret_cast<const float4u*>(span + c), reinterpret_cast<float4u*>(row + c));
+        for (; c < n; c++) row[c] = span[c];
+        __syncthreads();
+        if (first)
+            for (uint32_t j = lane; j < k; j += kWave) {
+                const uint64_t at = indices[r * k + j] - c0;
+                if (at < n) span[at] = 0.f;
+            }
+    }
+}
+// Adding to what is there: a wave takes as many rows as it has lanes for, or one of more than 64 places.
+__global__ __launch_bounds__(256) void topk_bwd_add_kernel(const uint64_t* indices, const float* y_g, float* x_g, size_t rows,
+                                                           uint32_t cols, uint32_t k, int bits) {
+    const int lane = threadIdx.x % kWave;
+    const uint32_t wide = k < kWave ? k : kWave;  // entries of a row the wave takes at a time
+    const uint32_t per_wave = kWave / wide, mine = lane / wide, j_lane = lane % wide;
+    const uint64_t row_lanes = wide == kWave ? ~(uint64_t)0 : (((uint64_t)1 << wide) - 1) << (mine * wide % kWave);
+    for (size_t r0 = ((size_t)blockIdx.x * 4 + threadIdx.x / kWave) * per_wave; r0 < rows; r0 += (size_t)gridDim.x * 4 * per_wave) {
+        const size_t r = r0 + mine;
+        for (uint32_t j0 = 0; j0 < k; j0 += wide) {
+            if (j0) stores_done();
+            const bool live = mine < per_wave && r < rows && j0 + j_lane < k;
+            const size_t i = r * k + j0 + j_lane;
+            const uint64_t idx = live ? indices[i] : ~(uint64_t)0;
+            const bool here = idx < cols;
+            const uint32_t col = here ? (uint32_t)idx : 0u;
+            uint64_t same = same_lanes(col, bits, __ballot(here) & row_lanes);
+            if (!here) same = 0;
+            add_entries<false>(x_g + (here ? r : 0) * cols + col, here ? y_g[i] : 0.f, same, lane);
         }
     }
 }
@@ -494,20 +911,58 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
                "topk_fwd: an output overlaps another operand");
     DeviceGuard guard(ctx);
     const uint32_t c32 = (uint32_t)cols, k32 = (uint32_t)k;
-#define ZG_TOPK(NT, VPT)                                                                                                      \
-    hipLaunchKernelGGL((topk_kernel<NT, VPT>), dim3(row_grid(ceil_div_sz(rows, 256 / (NT)))), dim3(256), 0, ctx->stream, x, values, \
+#define ZG_TOPK(NT, VPT, BEYOND)                                                                                      \
+    hipLaunchKernelGGL((topk_kernel<NT, VPT, BEYOND>), dim3(grid(256 / (NT))), dim3(256), 0, ctx->stream, x, values,       \
                        indices, rows, c32, k32)
-    // A wave per row up to 2048 columns, as far as its 256 groups can bound k; a workgroup per row beyond.
-    if (cols <= 2048 && k <= 128) {
-        if (cols <= 256) ZG_TOPK(64, 1);
-        else if (cols <= 512) ZG_TOPK(64, 2);
-        else if (cols <= 1024) ZG_TOPK(64, 4);
-        else ZG_TOPK(64, 8);
-    } else if (cols <= 2048) {
-        ZG_TOPK(256, 2);
-    } else {
-        ZG_TOPK(256, 8);
+    // as many workgroups as the compute units hold, with the same number of rows each
+    auto grid = [&](size_t per_block) {
+        const size_t blocks = ceil_div_sz(rows, per_block), most = (size_t)ctx->n_cu * 4;
+        return (unsigned)ceil_div_sz(blocks, ceil_div_sz(blocks, most));
+    };
+    // A few long rows are cut into segments, which takes two launches (64 of 128000: 1 row 16 us against 39 us with a workgroup per
+    // row, 64 rows 26 against 43).  Up to 32000 columns both take the same time, and from k = 256 on the second launch has too much
+    // to sort (256 of 128000 in 64 rows: 66 against 53 us).
+    if (rows <= 64 && k <= 128 && cols >= 8 * (size_t)kTopkSegment) {
+        uint32_t n_seg = (uint32_t)ceil_div_sz(cols, kTopkSegment);
+        const uint32_t len = (uint32_t)((ceil_div_sz(cols, n_seg) + 3) & ~(size_t)3);  // at most kTopkSegment, as n_seg segments reach
+        n_seg = (uint32_t)ceil_div_sz(cols, len);
+        if (cols - (size_t)(n_seg - 1) * len >= k) {
+            uint64_t* keys = (uint64_t*)workspace(ctx, rows * n_seg * k * sizeof(uint64_t));
+            if (!keys) return ZG_HIP_EOOM;
+            hipLaunchKernelGGL(topk_segments_kernel, dim3((unsigned)(rows * n_seg)), dim3(256), 0, ctx->stream, x, keys, c32, k32, len, n_seg);
+            ZG_LAUNCH_CHECK();
+            hipLaunchKernelGGL(topk_join_kernel, dim3((unsigned)rows), dim3(256), 0, ctx->stream, x, keys, values, indices, c32, k32, n_seg);
+            ZG_LAUNCH_CHECK();
+            return ZG_HIP_OK;
+        }
     }
+    // A wave per row as far as its 256 groups can bound k and there are rows enough to fill the compute units (or the row is
+    // short): its waves never wait for each other (64 of 8192 in 8192 rows: 64 us against 97 us with a workgroup per row).  A
+    // workgroup per row else.
+#define ZG_TOPK_SHORT(L, KPL)                                                                                                    \
+    hipLaunchKernelGGL((topk_short_kernel<L, KPL>), dim3((unsigned)ceil_div_sz(rows, 256 / (L))), dim3(256), 0, ctx->stream, x,      \
+                       values, indices, rows, c32, k32)
+    if (cols <= 256 && k <= 16 && rows < ((size_t)1 << 34)) {
+        if (cols <= 16) ZG_TOPK_SHORT(4, 4);
+        else if (cols <= 64) ZG_TOPK_SHORT(16, 4);
+        else if (cols <= 128) ZG_TOPK_SHORT(16, 8);
+        else ZG_TOPK_SHORT(16, 16);
+    } else if (k <= 128 && (cols <= 2048 || rows >= (size_t)ctx->n_cu * 8)) {
+        if (cols <= 256) ZG_TOPK(64, 1, false);
+        else if (cols <= 512) ZG_TOPK(64, 2, false);
+        else if (cols <= 1024) ZG_TOPK(64, 4, false);
+        else if (cols <= 2048) ZG_TOPK(64, 8, false);
+        else ZG_TOPK(64, 8, true);
+    } else if (cols <= 2048) {
+        ZG_TOPK(256, 2, false);
+    } else if (cols <= 4096) {
+        ZG_TOPK(256, 4, false);
+    } else if (cols <= 8192) {
+        ZG_TOPK(256, 8, false);
+    } else {
+        ZG_TOPK(256, 8, true);
+    }
+#undef ZG_TOPK_SHORT
 #undef ZG_TOPK
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
@@ -525,10 +980,23 @@ ZG_API int zg_hip_topk_bwd(zg_hip_ctx* ctx, const uint64_t* indices, const float
     ZG_REQUIRE(!ranges_overlap(x_g, rows * cols * 4, y_g, rows * k * 4) && !ranges_overlap(x_g, rows * cols * 4, indices, rows * k * 8),
                "topk_bwd: x_g overlaps an input");
     DeviceGuard guard(ctx);
-    if (accumulate)
-        hipLaunchKernelGGL(topk_bwd_kernel<true>, dim3(row_grid(rows)), dim3(kBlock), 0, ctx->stream, indices, y_g, x_g, rows, cols, k);
-    else
-        hipLaunchKernelGGL(topk_bwd_kernel<false>, dim3(row_grid(rows)), dim3(kBlock), 0, ctx->stream, indices, y_g, x_g, rows, cols, k);
+    const uint32_t c32 = (uint32_t)cols, k32 = (uint32_t)k;
+    int bits = 1;  // of a column
+    while (((size_t)1 << bits) < cols) bits++;
+    if (accumulate) {
+        const size_t per_wave = k < kWave ? kWave / k : 1;
+        hipLaunchKernelGGL(topk_bwd_add_kernel, dim3(row_grid(ceil_div_sz(rows, 4 * per_wave))), dim3(256), 0, ctx->stream, indices, y_g,
+                           x_g, rows, c32, k32, bits);
+    } else if (cols <= 256 && k <= 16 && rows < ((size_t)1 << 34)) {
+        const dim3 grid((unsigned)ceil_div_sz(rows, 16));
+        if (cols <= 64) hipLaunchKernelGGL(topk_bwd_short_kernel<1>, grid, dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32);
+        else if (cols <= 128) hipLaunchKernelGGL(topk_bwd_short_kernel<2>, grid, dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32);
+        else hipLaunchKernelGGL(topk_bwd_short_kernel<4>, grid, dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32);
+    } else {
+        const uint32_t spans = (uint32_t)ceil_div_sz(cols, kBwdSpan);
+        hipLaunchKernelGGL(topk_bwd_kernel, dim3(row_grid(ceil_div_sz(rows * spans, 4))), dim3(256), 0, ctx->stream, indices, y_g, x_g,
+                           rows, c32, k32, spans, bits < 12 ? bits : 12);
+    }
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
 }
