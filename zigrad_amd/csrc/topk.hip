@@ -592,14 +592,6 @@ __global__ __launch_bounds__(256) void topk_short_kernel(const float* x, float* 
 // A row's chosen places in LDS: entry j holds its column (kNoCol: none), and only the first of the entries that name a
 // column speaks for it.
 constexpr uint32_t kNoCol = 0xffffffffu;
-__device__ __forceinline__ bool speaks(const uint32_t* col, int j) {
-    const uint32_t c = col[j];
-    if (c == kNoCol) return false;
-    for (int i = 0; i < j; i++)
-        if (col[i] == c) return false;
-    return true;
-}
-
 // The gradient of a selection, dense, for short rows and few places: 16 lanes share a row, every lane compares its columns with each
 // chosen one (the gradients of a repeated index are added in the order of j by themselves).
 template <int P>  // pieces of four columns a lane has: 64 P columns at most
@@ -730,25 +722,14 @@ __global__ __launch_bounds__(256) void topk_bwd_add_kernel(const uint64_t* indic
 }
 
 // ------------------------------------------------------------------------------------------------
-// distillation
+// Distillation.  With c = log2(e) / T and m, tm the largest logit of the student and the teacher:
+//   e_c = 2^((x_c - m) c), s = sum e_c, p_c = e_c / s      f_j = 2^((t_j - tm) c), S = sum f_j, q_j = f_j / S
+//   row_loss = T^2 (sum_j f_j ((t_j - tm) - (x_{i_j} - m)) / T / S - log S + log s)
+// A row's logits are read once, into registers, by 16 lanes, a wave, or a workgroup of 256 or 1024, by its length (rows of
+// more than 65536 columns are read twice); the maxima, then all sums, take one reduction each.  For the gradient the q_j go into a
+// stretch of LDS laid out like the row, from where every thread takes what belongs to its columns: the gradient leaves in whole
+// 16-byte pieces, written once, and a class that is named twice gets both shares, added in the order of j by one wave.
 // ------------------------------------------------------------------------------------------------
-struct MaxF {
-    using Acc = float;
-    static __device__ __forceinline__ Acc init() { return -INFINITY; }
-    static __device__ __forceinline__ Acc combine(Acc a, Acc b) { return fmaxf(a, b); }
-    static __device__ __forceinline__ Acc shfl_xor(Acc a, int m) { return __shfl_xor(a, m, kWave); }
-};
-template <class P>
-__device__ __forceinline__ typename P::Acc block_all(typename P::Acc v, typename P::Acc* smem) {
-    v = block_reduce<P>(v, smem);
-    __syncthreads();
-    if (threadIdx.x == 0) smem[0] = v;
-    __syncthreads();
-    v = smem[0];
-    __syncthreads();
-    return v;
-}
-
 struct DistillArgs {
     const float* x;
     const float* t;
@@ -757,116 +738,512 @@ struct DistillArgs {
     float* stats;
     float* row_loss;
     float* grad;
-    size_t rows, cols, k;
-    float temp, inv_temp, mean;
+    size_t rows;
+    uint32_t cols, k;
+    float temp, inv_temp, scale, mean;  // scale = log2(e) / temp
 };
 
-// FWD: statistics and loss; BWD: gradient, added when ACC
+// the hardware's 2^x: off by a step at most, which with the roundings of its argument is what exp(x) of a library has lost as well
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The largest of `top` and the sum of each of `sum` over the NT threads of a row, in all of them.  `smem`: 4 (NT / 64) floats.
+template <int NT, int N>
+__device__ __forceinline__ void row_sums(float (&sum)[N], float* smem) {
+    constexpr int W = NT < kWave ? NT : kWave;
+#pragma unroll
+    for (int m = W / 2; m >= 1; m >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; i++) sum[i] += __shfl_xor(sum[i], m, kWave);
+    if constexpr (NT > kWave) {
+        const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+        __syncthreads();
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < N; i++) smem[i * (NT / kWave) + wave] = sum[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float all = smem[i * (NT / kWave)];
+            for (int w = 1; w < NT / kWave; w++) all += smem[i * (NT / kWave) + w];
+            sum[i] = all;
+        }
+    }
+}
+template <int NT, int N>
+__device__ __forceinline__ void row_maxima(float (&top)[N], float* smem) {
+    constexpr int W = NT < kWave ? NT : kWave;
+#pragma unroll
+    for (int m = W / 2; m >= 1; m >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; i++) top[i] = fmaxf(top[i], __shfl_xor(top[i], m, kWave));
+    if constexpr (NT > kWave) {
+        const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+        __syncthreads();
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < N; i++) smem[i * (NT / kWave) + wave] = top[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float all = smem[i * (NT / kWave)];
+            for (int w = 1; w < NT / kWave; w++) all = fmaxf(all, smem[i * (NT / kWave) + w]);
+            top[i] = all;
+        }
+    }
+}
+
+// What the row's numbers come to once they are known: the statistics, the loss and the factors of the gradient.
+struct RowResult {
+    float m, ls, loss;      // stats and row_loss
+    float inv_s, inv_S, f;  // p = e inv_s, q = f_j inv_S, gradient = f (p - q)
+    bool empty;
+};
+// m, tm: the maxima as found (-inf: nothing above); s, S, W: the sums, taken from 0 where a maximum is -inf.  With FWD false m and ls
+// are the row's statistics and s, W are not looked at.
+template <bool FWD>
+__device__ __forceinline__ RowResult row_result(const DistillArgs& a, float w, float m, float ls, float s, float S, float W) {
+    RowResult r;
+    r.m = m;
+    r.ls = ls;
+    if (FWD) {
+        r.ls = logf(s);
+        if (m == -INFINITY) {
+            if (s != 0.f) r.m = NAN;  // NaNs among logits of -inf
+            else r.ls = 0.f;
+        }
+        r.inv_s = __fdiv_rn(1.f, s);
+    } else {
+        r.inv_s = expf(-ls);
+    }
+    r.empty = S == 0.f || r.m == -INFINITY;
+    r.loss = r.empty ? 0.f : (W / S - logf(S) + r.ls) * (a.temp * a.temp);
+    r.inv_S = __fdiv_rn(1.f, S);
+    r.f = w * a.temp;
+    return r;
+}
+
+// An entry of the teacher: its column (kNoCol: padding) and its logit.
+__device__ __forceinline__ void teacher_entry(const DistillArgs& a, size_t r, uint32_t j, uint32_t& col, float& t) {
+    const bool live = j < a.k;
+    const uint64_t c = live ? a.idx[r * a.k + j] : ~(uint64_t)0;
+    col = c < a.cols ? (uint32_t)c : kNoCol;
+    t = col != kNoCol ? a.t[r * a.k + j] : -INFINITY;
+}
+// f_j and its part of W: x is the student's logit of the entry's class
+__device__ __forceinline__ void teacher_terms(const DistillArgs& a, float t, float x, float from_t, float from_x, float& f, float& part) {
+    f = exp2_fast((t - from_t) * a.scale);
+    part = f != 0.f ? f * (((t - from_t) - (x - from_x)) * a.inv_temp) : 0.f;
+}
+
+// Short rows with at most 16 entries: 16 lanes a row, P pieces of four columns and an entry each.  ONE: the only workgroup, which also
+// adds up the loss.
+template <int NTB, int P, bool FWD, bool BWD, bool ACC, bool ONE>
+__global__ __launch_bounds__(NTB) void distill_short_kernel(DistillArgs a, float* loss) {
+    const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
+    float total = 0.f;
+    for (size_t r0 = (size_t)blockIdx.x * (NTB / 16); r0 < a.rows; r0 += (size_t)gridDim.x * (NTB / 16)) {
+        const size_t r = r0 + group;
+        const bool live = r < a.rows;
+        const float w = live ? (a.w ? a.w[r] : a.mean) : 0.f;
+        const bool real = live && w != 0.f;
+        const float* x = a.x + (real ? r : 0) * a.cols;
+        float* grad = BWD ? a.grad + (real ? r : 0) * a.cols : nullptr;
+        float v[4 * P], old[4 * P];
+#pragma unroll
+        for (int i = 0; i < 4 * P; i++) {
+            const uint32_t c = (i / 4) * 64 + 4 * lane + i % 4;
+            v[i] = real && c < a.cols ? x[c] : -INFINITY;
+            old[i] = ACC && real && c < a.cols ? grad[c] : 0.f;
+        }
+        uint32_t col = kNoCol;
+        float t = -INFINITY;
+        if (real) teacher_entry(a, r, lane, col, t);
+        const float xe = FWD && col != kNoCol ? x[col] : 0.f;
+        float top[2] = {t, -INFINITY};
+        if (FWD) {
+#pragma unroll
+            for (int i = 0; i < 4 * P; i++) top[1] = fmaxf(top[1], v[i]);
+        }
+        row_maxima<16, 2>(top, nullptr);
+        const float m = FWD ? top[1] : (real ? a.stats[2 * r] : 0.f), ls = FWD ? 0.f : (real ? a.stats[2 * r + 1] : 0.f);
+        const float from_x = m == -INFINITY ? 0.f : m, from_t = top[0] == -INFINITY ? 0.f : top[0];
+        float sum[3] = {0.f, 0.f, 0.f};  // s, S, W
+#pragma unroll
+        for (int i = 0; i < 4 * P; i++) {
+            v[i] = exp2_fast((v[i] - from_x) * a.scale);
+            sum[0] += v[i];
+        }
+        float f, part;
+        teacher_terms(a, t, xe, from_t, from_x, f, part);
+        sum[1] = f;
+        sum[2] = part;
+        row_sums<16, 3>(sum, nullptr);
+        const RowResult res = row_result<FWD>(a, w, m, ls, sum[0], sum[1], sum[2]);
+        if (FWD && live && lane == 0) {
+            a.stats[2 * r] = real ? res.m : 0.f;
+            a.stats[2 * r + 1] = real ? res.ls : 0.f;
+            const float l = real ? res.loss : 0.f;
+            a.row_loss[r] = l;
+            if (ONE && real) total += a.w ? w * l : l;
+        }
+        if (BWD) {
+            const bool zero = !real || res.empty;
+            float share[4 * P];
+#pragma unroll
+            for (int i = 0; i < 4 * P; i++) share[i] = 0.f;
+            const float q = f * res.inv_S;
+            for (uint32_t j = 0; j < a.k; j++) {
+                const uint32_t at = (uint32_t)__shfl((int)col, j, 16) - 4 * lane;
+                const float qj = __shfl(q, j, 16);
+#pragma unroll
+                for (int i = 0; i < 4 * P; i++) share[i] = at == (uint32_t)((i / 4) * 64 + i % 4) ? share[i] + qj : share[i];
+            }
+            if (live && !(ACC && zero)) {
+                float* g = a.grad + r * a.cols;
+#pragma unroll
+                for (int i = 0; i < 4 * P; i++) {
+                    const uint32_t c = (i / 4) * 64 + 4 * lane + i % 4;
+                    const float d = zero ? 0.f : res.f * (v[i] * res.inv_s - share[i]);
+                    if (c < a.cols) g[c] = ACC ? old[i] + d : d;
+                }
+            }
+        }
+    }
+    if constexpr (ONE) {
+        __shared__ float smem[NTB / kWave];
+        total = block_reduce<SumAcc>(total, smem);
+        if (threadIdx.x == 0) *loss = a.w ? total : __fdiv_rn(total, (float)a.rows);
+    }
+}
+
+// The q_j of the columns [c0, c0 + n) into the stretch of zeros `span`, by one wave, in the order of j.
+__device__ __forceinline__ void span_shares(float* span, const uint32_t* col, const float* q, uint32_t k, uint32_t c0, uint32_t n, int bits,
+                                            int lane) {
+    for (uint32_t j0 = 0; j0 < k; j0 += kWave) {
+        const uint32_t at = (j0 + lane < k ? col[j0 + lane] : kNoCol) - c0;
+        const bool here = at < n;  // (kNoCol - c0 is beyond: rows are shorter than 2^31)
+        const uint64_t heres = __ballot(here);
+        if (!heres) continue;
+        uint64_t same = same_lanes(here ? at : 0u, bits, heres);
+        if (!here) same = 0;
+        add_entries<false>(span + (here ? at : 0u), here ? q[j0 + lane] : 0.f, same, lane);
+        select_sync<kWave>();
+    }
+}
+// four values of the gradient; clears what it takes from the stretch
+__device__ __forceinline__ float4u take_shares(float* at) {
+    const float4 s = *reinterpret_cast<const float4*>(at);
+    if (s.x != 0.f || s.y != 0.f || s.z != 0.f || s.w != 0.f) *reinterpret_cast<float4*>(at) = make_float4(0.f, 0.f, 0.f, 0.f);
+    return float4u{s.x, s.y, s.z, s.w};
+}
+
+// NT threads a row (a wave: four rows a workgroup), which they hold in VPT pieces of four columns each; the gradient leaves UP pieces
+// per thread at a time.
+template <int NT, int VPT, int UP, bool FWD, bool BWD, bool ACC>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_row_kernel(DistillArgs a) {
+    constexpr int kRows = NT < 256 ? 256 / NT : 1;
+    constexpr uint32_t kSpan = 4 * NT * UP;
+    constexpr int kBits = 2 + (NT == 64 ? 6 : NT == 256 ? 8 : 10) + (UP == 1 ? 0 : UP == 2 ? 1 : UP == 4 ? 2 : 3);
+    constexpr int kEntries = (kMaxK + NT - 1) / NT;
+    __shared__ __attribute__((aligned(16))) float span_mem[BWD ? kRows * kSpan : 4];
+    __shared__ uint32_t col_mem[BWD ? kRows * kMaxK : 1];
+    __shared__ float q_mem[BWD ? kRows * kMaxK : 1];
+    __shared__ float smem[NT > kWave ? 3 * (NT / kWave) : 1];
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+    const int sub = NT == kWave ? wave : 0, tid = threadIdx.x % NT;
+    float* const span = span_mem + (BWD ? sub * kSpan : 0);
+    uint32_t* const col_of = col_mem + (BWD ? sub * kMaxK : 0);
+    float* const q_of = q_mem + (BWD ? sub * kMaxK : 0);
+    const size_t r = (size_t)blockIdx.x * kRows + sub;
+    if (r >= a.rows) return;  // only waves that own a row of their own: no barrier is missed
+    const uint32_t cols = a.cols, whole = cols & ~3u;
+    const float* x = a.x + r * cols;
+    float* grad = BWD ? a.grad + r * cols : nullptr;
+    const float w = a.w ? a.w[r] : a.mean;
+    if (w == 0.f) {
+        if (FWD && tid == 0) {
+            a.stats[2 * r] = a.stats[2 * r + 1] = 0.f;
+            a.row_loss[r] = 0.f;
+        }
+        if (BWD && !ACC) {
+            for (uint32_t c = 4 * tid; c < whole; c += 4 * NT) *reinterpret_cast<float4u*>(grad + c) = float4u{0.f, 0.f, 0.f, 0.f};
+            if (whole + tid < cols) grad[whole + tid] = 0.f;
+        }
+        return;
+    }
+    float4u v[VPT];
+#pragma unroll
+    for (int u = 0; u < VPT; u++) v[u] = row_piece(x, bytes_from(0, whole), 16 * (tid + u * NT));
+    const float tail = whole + tid < cols ? x[whole + tid] : -INFINITY;  // of the first threads
+    uint32_t col[kEntries];
+    float t[kEntries], xe[kEntries];
+    float top[2] = {-INFINITY, tail};
+#pragma unroll
+    for (int i = 0; i < kEntries; i++) {
+        if (i == 0 || i * NT < (int)a.k) {
+            teacher_entry(a, r, tid + i * NT, col[i], t[i]);
+            xe[i] = FWD && col[i] != kNoCol ? x[col[i]] : 0.f;
+            top[0] = fmaxf(top[0], t[i]);
+        } else {
+            col[i] = kNoCol;
+            t[i] = -INFINITY;
+            xe[i] = 0.f;
+        }
+    }
+    if (BWD) {
+#pragma unroll
+        for (int u = 0; u < UP; u++) *reinterpret_cast<float4*>(span + 4 * (tid + u * NT)) = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float m, ls;
+    if (FWD) {
+#pragma unroll
+        for (int u = 0; u < VPT; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) top[1] = fmaxf(top[1], v[u][e]);
+        row_maxima<NT, 2>(top, smem);
+        m = top[1];
+        ls = 0.f;
+    } else {
+        float one[1] = {top[0]};
+        row_maxima<NT, 1>(one, smem);
+        top[0] = one[0];
+        m = a.stats[2 * r];
+        ls = a.stats[2 * r + 1];
+    }
+    const float from_x = m == -INFINITY ? 0.f : m, from_t = top[0] == -INFINITY ? 0.f : top[0];
+    float sum[3] = {0.f, 0.f, 0.f};
+    float f[kEntries];
+#pragma unroll
+    for (int i = 0; i < kEntries; i++) {
+        float part;
+        teacher_terms(a, t[i], xe[i], from_t, from_x, f[i], part);
+        sum[0] += f[i];
+        sum[1] += part;
+    }
+#pragma unroll
+    for (int u = 0; u < VPT; u++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[u][e] = exp2_fast((v[u][e] - from_x) * a.scale);
+        sum[2] += (v[u][0] + v[u][1]) + (v[u][2] + v[u][3]);
+    }
+    const float tail_e = exp2_fast((tail - from_x) * a.scale);
+    sum[2] += tail_e;
+    if (FWD) {
+        row_sums<NT, 3>(sum, smem);
+    } else {
+        float one[1] = {sum[0]};
+        row_sums<NT, 1>(one, smem);
+        sum[0] = one[0];
+    }
+    const RowResult res = row_result<FWD>(a, w, m, ls, sum[2], sum[0], sum[1]);
+    if (FWD && tid == 0) {
+        a.stats[2 * r] = res.m;
+        a.stats[2 * r + 1] = res.ls;
+        a.row_loss[r] = res.loss;
+    }
+    if constexpr (BWD) {
+        if (ACC && res.empty) return;
+#pragma unroll
+        for (int i = 0; i < kEntries; i++)
+            if (tid + i * NT < kMaxK) {
+                col_of[tid + i * NT] = col[i];
+                q_of[tid + i * NT] = f[i] * res.inv_S;
+            }
+        const float fac = res.empty ? 0.f : res.f, inv_s = res.inv_s;
+        float4u share_t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ph = 0; ph < VPT / UP; ph++) {
+            const uint32_t c0 = ph * kSpan;
+            if (c0 >= cols) break;
+            select_sync<NT>();
+            if (NT == kWave || wave == 0)
+                span_shares(span, col_of, q_of, a.k, c0, kSpan, kBits, threadIdx.x % kWave);
+            float4u old[UP];
+            if (ACC) {
+#pragma unroll
+                for (int u = 0; u < UP; u++) old[u] = row_piece(grad + c0, bytes_from(c0, whole), 16 * (tid + u * NT));
+            }
+            select_sync<NT>();
+            if (whole >= c0 && whole - c0 < kSpan && whole + tid < cols) share_t[0] = span[whole - c0 + tid];
+#pragma unroll
+            for (int u = 0; u < UP; u++) {
+                const uint32_t c = 4 * (tid + u * NT);
+                if (c0 + c >= whole) continue;  // the tail's shares are for the first threads
+                const float4u q = take_shares(span + c);
+                float4u g;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float d = res.empty ? 0.f : fac * (v[ph * UP + u][e] * inv_s - q[e]);
+                    g[e] = ACC ? old[u][e] + d : d;
+                }
+                __builtin_nontemporal_store(g, reinterpret_cast<float4u*>(grad + c0 + c));
+            }
+        }
+        if (whole + tid < cols) {
+            const float d = res.empty ? 0.f : fac * (tail_e * inv_s - share_t[0]);
+            grad[whole + tid] = ACC ? grad[whole + tid] + d : d;
+        }
+    }
+}
+
+// Rows of any length: a workgroup reads the row once for its statistics (a running maximum, the sum rescaled when it grows) and once
+// more for its gradient.
+constexpr int kStreamNT = 1024;
 template <bool FWD, bool BWD, bool ACC>
-__global__ __launch_bounds__(kBlock) void distill_kernel(DistillArgs a) {
-    __shared__ float smem[kBlock / kWave];
-    __shared__ uint32_t col[kMaxK];
-    __shared__ float q[kMaxK];
+__global__ __launch_bounds__(kStreamNT) void distill_stream_kernel(DistillArgs a) {
+    constexpr int NT = kStreamNT, UP = 2;
+    constexpr uint32_t kSpan = 4 * NT * UP;
+    constexpr int kBits = 13;
+    __shared__ __attribute__((aligned(16))) float span[BWD ? kSpan : 4];
+    __shared__ uint32_t col_of[BWD ? kMaxK : 1];
+    __shared__ float q_of[BWD ? kMaxK : 1];
+    __shared__ float smem[3 * (NT / kWave)];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+    const uint32_t cols = a.cols, whole = cols & ~3u;
     for (size_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const float* x = a.x + r * a.cols;
-        float* grad = BWD ? a.grad + r * a.cols : nullptr;
+        const float* x = a.x + r * cols;
+        float* grad = BWD ? a.grad + r * cols : nullptr;
         const float w = a.w ? a.w[r] : a.mean;
+        __syncthreads();
         if (w == 0.f) {
-            if (FWD && threadIdx.x == 0) {
+            if (FWD && tid == 0) {
                 a.stats[2 * r] = a.stats[2 * r + 1] = 0.f;
                 a.row_loss[r] = 0.f;
             }
             if (BWD && !ACC)
-                for (size_t c = threadIdx.x; c < a.cols; c += kBlock) grad[c] = 0.f;
+                for (uint32_t c = tid; c < cols; c += NT) grad[c] = 0.f;
             continue;
         }
-        // the student's statistics
-        float m, ls;
+        uint32_t col;
+        float t;
+        teacher_entry(a, r, tid, col, t);
+        const float xe = FWD && col != kNoCol ? x[col] : 0.f;
+        const float tail = whole + tid < cols ? x[whole + tid] : -INFINITY;
+        float m = -INFINITY, s = 0.f, ls = 0.f;
+        float top[2] = {t, tail};
         if (FWD) {
-            float mx = -INFINITY;
-            for (size_t c = threadIdx.x; c < a.cols; c += kBlock) mx = fmaxf(mx, x[c]);
-            m = block_all<MaxF>(mx, smem);
-            float s = 0.f;
-            const float from = m == -INFINITY ? 0.f : m;
-            for (size_t c = threadIdx.x; c < a.cols; c += kBlock) s += expf((x[c] - from) * a.inv_temp);
-            s = block_all<SumAcc>(s, smem);
-            ls = logf(s);
-            if (m == -INFINITY) {
-                if (s != 0.f) m = NAN;  // NaNs among logits of -inf
-                else ls = 0.f;
+            float mine = -INFINITY;  // this thread's maximum, and its sum from there
+            for (uint32_t c0 = 0; c0 < whole; c0 += 2 * kSpan) {
+                float4u v[2 * UP];
+#pragma unroll
+                for (int u = 0; u < 2 * UP; u++) v[u] = row_piece(x + c0, bytes_from(c0, whole), 16 * (tid + u * NT));
+                float mx = v[0][0];
+#pragma unroll
+                for (int u = 0; u < 2 * UP; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx = fmaxf(mx, v[u][e]);
+                if (mx > mine) {
+                    s = mine == -INFINITY ? s : s * exp2_fast((mine - mx) * a.scale);
+                    mine = mx;
+                }
+                const float from = mine == -INFINITY ? 0.f : mine;
+#pragma unroll
+                for (int u = 0; u < 2 * UP; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s += exp2_fast((v[u][e] - from) * a.scale);
             }
-            if (threadIdx.x == 0) {
-                a.stats[2 * r] = m;
-                a.stats[2 * r + 1] = ls;
-            }
+            top[1] = fmaxf(top[1], mine);
+            row_maxima<NT, 2>(top, smem);
+            m = top[1];
+            if (mine != -INFINITY) s *= exp2_fast((mine - m) * a.scale);
         } else {
+            float one[1] = {top[0]};
+            row_maxima<NT, 1>(one, smem);
+            top[0] = one[0];
             m = a.stats[2 * r];
             ls = a.stats[2 * r + 1];
         }
-        // the teacher's distribution
-        float tm = -INFINITY;
-        for (size_t j = threadIdx.x; j < a.k; j += kBlock) {
-            const uint64_t c = a.idx[r * a.k + j];
-            const bool held = c < a.cols;
-            col[j] = held ? (uint32_t)c : kNoCol;
-            if (held) tm = fmaxf(tm, a.t[r * a.k + j]);
+        const float from_x = m == -INFINITY ? 0.f : m, from_t = top[0] == -INFINITY ? 0.f : top[0];
+        const float tail_e = exp2_fast((tail - from_x) * a.scale);
+        float f, part;
+        teacher_terms(a, t, xe, from_t, from_x, f, part);
+        float sum[3] = {f, part, s + tail_e};
+        row_sums<NT, 3>(sum, smem);
+        const RowResult res = row_result<FWD>(a, w, m, ls, sum[2], sum[0], sum[1]);
+        if (FWD && tid == 0) {
+            a.stats[2 * r] = res.m;
+            a.stats[2 * r + 1] = res.ls;
+            a.row_loss[r] = res.loss;
         }
-        tm = block_all<MaxF>(tm, smem);
-        const float t_from = tm == -INFINITY ? 0.f : tm;
-        float ts = 0.f;
-        for (size_t j = threadIdx.x; j < a.k; j += kBlock) {
-            q[j] = col[j] != kNoCol ? expf((a.t[r * a.k + j] - t_from) * a.inv_temp) : 0.f;
-            ts += q[j];
-        }
-        ts = block_all<SumAcc>(ts, smem);
-        const bool empty = ts == 0.f || m == -INFINITY;
-        if (FWD) {
-            const float lts = logf(ts);
-            float part = 0.f;
-            for (size_t j = threadIdx.x; j < a.k; j += kBlock)
-                if (q[j] != 0.f && !empty) {
-                    const float log_q = (a.t[r * a.k + j] - t_from) * a.inv_temp - lts;
-                    const float log_p = (x[col[j]] - m) * a.inv_temp - ls;
-                    part += q[j] / ts * (log_q - log_p);
+        if constexpr (BWD) {
+            if (ACC && res.empty) continue;
+            if (tid < kMaxK) {
+                col_of[tid] = col;
+                q_of[tid] = f * res.inv_S;
+            }
+#pragma unroll
+            for (int u = 0; u < UP; u++) *reinterpret_cast<float4*>(span + 4 * (tid + u * NT)) = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t c0 = 0; c0 < cols; c0 += kSpan) {
+                float4u v[UP], old[UP];
+#pragma unroll
+                for (int u = 0; u < UP; u++) v[u] = row_piece(x + c0, bytes_from(c0, whole), 16 * (tid + u * NT));
+                if (ACC) {
+#pragma unroll
+                    for (int u = 0; u < UP; u++) old[u] = row_piece(grad + c0, bytes_from(c0, whole), 16 * (tid + u * NT));
                 }
-            part = block_all<SumAcc>(part, smem);
-            if (threadIdx.x == 0) a.row_loss[r] = empty ? 0.f : part * a.temp * a.temp;
-        }
-        if (BWD) {
-            if (empty) {
-                if (!ACC)
-                    for (size_t c = threadIdx.x; c < a.cols; c += kBlock) grad[c] = 0.f;
                 __syncthreads();
-                continue;
-            }
-            const float f = w * a.temp;
-            __syncthreads();
-            float old[kMaxK / kBlock];
-            for (int u = 0; u < kMaxK / kBlock; u++) {
-                const int j = threadIdx.x + u * kBlock;
-                old[u] = (ACC && j < (int)a.k && col[j] != kNoCol) ? grad[col[j]] : 0.f;
-            }
-            __syncthreads();
-            for (size_t c = threadIdx.x; c < a.cols; c += kBlock) {
-                const float v = f * expf((x[c] - m) * a.inv_temp - ls);
-                grad[c] = ACC ? grad[c] + v : v;
-            }
-            __syncthreads();
-            for (int u = 0; u < kMaxK / kBlock; u++) {
-                const int j = threadIdx.x + u * kBlock;
-                if (j >= (int)a.k || !speaks(col, j)) continue;
-                float sum = 0.f;
-                for (int i = j; i < (int)a.k; i++)
-                    if (col[i] == col[j]) sum += q[i];
-                const float v = f * (expf((x[col[j]] - m) * a.inv_temp - ls) - sum / ts);
-                grad[col[j]] = ACC ? old[u] + v : v;
+                if (wave == 0) span_shares(span, col_of, q_of, a.k, c0, kSpan, kBits, tid);
+                __syncthreads();
+                if (whole >= c0 && whole - c0 < kSpan && whole + tid < cols) {
+                    const float d = res.empty ? 0.f : res.f * (tail_e * res.inv_s - span[whole - c0 + tid]);
+                    grad[whole + tid] = ACC ? grad[whole + tid] + d : d;
+                }
+#pragma unroll
+                for (int u = 0; u < UP; u++) {
+                    const uint32_t c = 4 * (tid + u * NT);
+                    if (c0 + c >= whole) continue;
+                    const float4u q = take_shares(span + c);
+                    float4u g;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float d = res.empty ? 0.f : res.f * (exp2_fast((v[u][e] - from_x) * a.scale) * res.inv_s - q[e]);
+                        g[e] = ACC ? old[u][e] + d : d;
+                    }
+                    __builtin_nontemporal_store(g, reinterpret_cast<float4u*>(grad + c0 + c));
+                }
             }
         }
-        __syncthreads();
     }
 }
 
 static unsigned row_grid(size_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
+
+template <bool FWD, bool BWD, bool ACC>
+static int distill_launch(zg_hip_ctx* ctx, const DistillArgs& a, float* loss, bool* summed) {
+    *summed = false;
+    if (a.cols <= 256 && a.k <= 16) {
+        const size_t blocks = ceil_div_sz(a.rows, 16);
+        const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
+        // a workgroup of its own for a small batch adds up the loss in the same launch
+        const bool one = FWD && a.rows <= 256;
+        *summed = one;
+#define ZG_SHORT(P)                                                                                                                  \
+    do {                                                                                                                             \
+        if (one) hipLaunchKernelGGL((distill_short_kernel<1024, P, FWD, BWD, ACC, FWD>), dim3(1), dim3(1024), 0, ctx->stream, a, loss); \
+        else hipLaunchKernelGGL((distill_short_kernel<256, P, FWD, BWD, ACC, false>), grid, dim3(256), 0, ctx->stream, a, loss);        \
+    } while (0)
+        if (a.cols <= 64) ZG_SHORT(1);
+        else if (a.cols <= 128) ZG_SHORT(2);
+        else ZG_SHORT(4);
+#undef ZG_SHORT
+        ZG_LAUNCH_CHECK();
+        return ZG_HIP_OK;
+    }
+#define ZG_ROWS(NT, VPT, UP)                                                                                                          \
+    hipLaunchKernelGGL((distill_row_kernel<NT, VPT, UP, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(a.rows, NT < 256 ? 256 / NT : 1)), \
+                       dim3(NT < 256 ? 256 : NT), 0, ctx->stream, a)
+    const bool fits = a.rows < 0x7fffffffull;
+    if (fits && a.cols <= 1024) ZG_ROWS(64, 4, 4);
+    else if (fits && a.cols <= 2048) ZG_ROWS(64, 8, 8);
+    else if (fits && a.cols <= 8192) ZG_ROWS(256, 8, 4);
+    else if (fits && a.cols <= 32768) ZG_ROWS(1024, 8, 2);
+    else if (fits && a.cols <= 65536) ZG_ROWS(1024, 16, 2);
+    else hipLaunchKernelGGL((distill_stream_kernel<FWD, BWD, ACC>), dim3(row_grid(a.rows)), dim3(kStreamNT), 0, ctx->stream, a);
+#undef ZG_ROWS
+    ZG_LAUNCH_CHECK();
+    return ZG_HIP_OK;
+}
+
 
 static int distill_check(const char* op, const float* logits, const float* teacher, const uint64_t* indices,
                          const float* row_weights, size_t rows, size_t cols, size_t k, float temperature) {
@@ -875,7 +1252,7 @@ static int distill_check(const char* op, const float* logits, const float* teach
     ZG_REQUIRE(cols < ((size_t)1 << 31), "%s: %zu columns", op, cols);
     ZG_REQUIRE(mul_sat(rows, cols) < ((size_t)1 << 60) && mul_sat(rows, k) < ((size_t)1 << 60), "%s: %zu rows", op, rows);
     ZG_REQUIRE(k >= 1 && k <= kMaxK, "%s: k = %zu is not in 1 .. %d", op, k, kMaxK);
-    ZG_REQUIRE(temperature > 0.f && temperature < INFINITY && 1.f / temperature < INFINITY, "%s: temperature %g", op, temperature);
+    ZG_REQUIRE(temperature > 0.f && temperature < INFINITY && 1.f / temperature < 1e38f, "%s: temperature %g", op, temperature);
     return ZG_HIP_OK;
 }
 // an output against the inputs of the loss
@@ -1023,16 +1400,18 @@ static int distill_entry(zg_hip_ctx* ctx, const char* op, const float* logits, c
                    "%s: grad overlaps another operand", op);
     }
     DeviceGuard guard(ctx);
-    DistillArgs a{logits, teacher, indices, row_weights, stats, row_loss, grad, rows, cols, k, temperature, 1.f / temperature,
-                  1.f / (float)rows};
-    const dim3 grid(row_grid(rows)), block(kBlock);
-    if (fwd && !bwd) hipLaunchKernelGGL((distill_kernel<true, false, false>), grid, block, 0, ctx->stream, a);
-    else if (!fwd && !accumulate) hipLaunchKernelGGL((distill_kernel<false, true, false>), grid, block, 0, ctx->stream, a);
-    else if (!fwd) hipLaunchKernelGGL((distill_kernel<false, true, true>), grid, block, 0, ctx->stream, a);
-    else if (!accumulate) hipLaunchKernelGGL((distill_kernel<true, true, false>), grid, block, 0, ctx->stream, a);
-    else hipLaunchKernelGGL((distill_kernel<true, true, true>), grid, block, 0, ctx->stream, a);
-    ZG_LAUNCH_CHECK();
-    return fwd ? distill_total(ctx, row_loss, row_weights, loss, rows) : ZG_HIP_OK;
+    const float inv_temp = 1.f / temperature;
+    DistillArgs a{logits, teacher, indices, row_weights, stats, row_loss, grad, rows, (uint32_t)cols, (uint32_t)k, temperature, inv_temp,
+                  inv_temp * 1.44269504088896340736f, 1.f / (float)rows};
+    bool summed = false;
+    int rc;
+    if (fwd && !bwd) rc = distill_launch<true, false, false>(ctx, a, loss, &summed);
+    else if (!fwd && !accumulate) rc = distill_launch<false, true, false>(ctx, a, loss, &summed);
+    else if (!fwd) rc = distill_launch<false, true, true>(ctx, a, loss, &summed);
+    else if (!accumulate) rc = distill_launch<true, true, false>(ctx, a, loss, &summed);
+    else rc = distill_launch<true, true, true>(ctx, a, loss, &summed);
+    if (rc || !fwd || summed) return rc;
+    return distill_total(ctx, row_loss, row_weights, loss, rows);
 }
 }  // namespace zg
 
