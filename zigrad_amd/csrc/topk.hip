@@ -850,10 +850,24 @@ __global__ __launch_bounds__(NTB) void distill_short_kernel(DistillArgs a, float
         float* grad = BWD ? a.grad + (real ? r : 0) * a.cols : nullptr;
         float v[4 * P], old[4 * P];
 #pragma unroll
-        for (int i = 0; i < 4 * P; i++) {
-            const uint32_t c = (i / 4) * 64 + 4 * lane + i % 4;
-            v[i] = real && c < a.cols ? x[c] : -INFINITY;
-            old[i] = ACC && real && c < a.cols ? grad[c] : 0.f;
+        for (int p = 0; p < P; p++) {
+            const uint32_t c = 64 * p + 4 * lane;
+            if (real && c + 4 <= a.cols) {
+                const float4u xs = *reinterpret_cast<const float4u*>(x + c);
+                float4u gs = {0.f, 0.f, 0.f, 0.f};
+                if (ACC) gs = *reinterpret_cast<const float4u*>(grad + c);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    v[4 * p + e] = xs[e];
+                    old[4 * p + e] = gs[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    v[4 * p + e] = real && c + e < a.cols ? x[c + e] : -INFINITY;
+                    old[4 * p + e] = ACC && real && c + e < a.cols ? grad[c + e] : 0.f;
+                }
+            }
         }
         uint32_t col = kNoCol;
         float t = -INFINITY;
@@ -901,10 +915,22 @@ __global__ __launch_bounds__(NTB) void distill_short_kernel(DistillArgs a, float
             if (live && !(ACC && zero)) {
                 float* g = a.grad + r * a.cols;
 #pragma unroll
-                for (int i = 0; i < 4 * P; i++) {
-                    const uint32_t c = (i / 4) * 64 + 4 * lane + i % 4;
-                    const float d = zero ? 0.f : res.f * (v[i] * res.inv_s - share[i]);
-                    if (c < a.cols) g[c] = ACC ? old[i] + d : d;
+                for (int p = 0; p < P; p++) {
+                    const uint32_t c = 64 * p + 4 * lane;
+                    float4u d;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int i = 4 * p + e;
+                        d[e] = zero ? 0.f : res.f * (v[i] * res.inv_s - share[i]);
+                        if (ACC) d[e] = old[i] + d[e];
+                    }
+                    if (c + 4 <= a.cols) {
+                        *reinterpret_cast<float4u*>(g + c) = d;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 3; e++)
+                            if (c + e < a.cols) g[c + e] = d[e];
+                    }
                 }
             }
         }
@@ -940,7 +966,7 @@ __device__ __forceinline__ float4u take_shares(float* at) {
 // NT threads a row (a wave: four rows a workgroup), which they hold in VPT pieces of four columns each; the gradient leaves UP pieces
 // per thread at a time.
 template <int NT, int VPT, int UP, bool FWD, bool BWD, bool ACC>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void distill_row_kernel(DistillArgs a) {
+__global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 && VPT == 8 && !ACC ? 8 : 1) void distill_row_kernel(DistillArgs a) {
     constexpr int kRows = NT < 256 ? 256 / NT : 1;
     constexpr uint32_t kSpan = 4 * NT * UP;
     constexpr int kBits = 2 + (NT == 64 ? 6 : NT == 256 ? 8 : 10) + (UP == 1 ? 0 : UP == 2 ? 1 : UP == 4 ? 2 : 3);
@@ -1232,7 +1258,7 @@ static int distill_launch(zg_hip_ctx* ctx, const DistillArgs& a, float* loss, bo
 #define ZG_ROWS(NT, VPT, UP)                                                                                                          \
     hipLaunchKernelGGL((distill_row_kernel<NT, VPT, UP, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(a.rows, NT < 256 ? 256 / NT : 1)), \
                        dim3(NT < 256 ? 256 : NT), 0, ctx->stream, a)
-    const bool fits = a.rows < 0x7fffffffull;
+    const bool fits = a.rows < 0x7fffffffull && (BWD || a.cols <= 32768);
     if (fits && a.cols <= 1024) ZG_ROWS(64, 4, 4);
     else if (fits && a.cols <= 2048) ZG_ROWS(64, 8, 8);
     else if (fits && a.cols <= 8192) ZG_ROWS(256, 8, 4);
