@@ -5,12 +5,13 @@ namespace zg {
 
 // ------------------------------------------------------------------------------------------------
 // expert_sort: a stable counting sort.  A workgroup owns a run of entries, each of its waves a run of those; counters are
-// integers in LDS, so their order of arrival changes nothing.
+// integers in LDS, so their order of arrival changes nothing.  Up to kSortAlone entries one workgroup does everything in a launch;
+// more are counted first, run by run, and every workgroup adds up for itself what lies before its run.  Latency bounds it
+// throughout (65536 entries are 1 MiB in and out).
 // ------------------------------------------------------------------------------------------------
 constexpr int kSortThreads = 512;
 constexpr int kSortWaves = kSortThreads / kWave;
-constexpr size_t kSortAlone = 8192;  // entries one workgroup orders in one launch
-constexpr size_t kSortMaxBlocks = 256;
+constexpr size_t kSortAlone = 2048;
 constexpr int kMaxExperts = ZG_HIP_EXPERTS_MAX;
 
 __global__ __launch_bounds__(kSortThreads) void expert_count_kernel(const uint64_t* experts, uint32_t* counts, size_t n,
@@ -32,11 +33,11 @@ __global__ __launch_bounds__(kSortThreads) void expert_place_kernel(const uint64
                                                                      uint64_t* offsets, uint64_t* slots, size_t n,
                                                                      size_t per_block, int n_experts) {
     extern __shared__ uint32_t mem[];
-    uint32_t* next = mem;                           // [wave][expert]: where the wave's next entry of the expert goes
-    uint32_t* base = mem + kSortWaves * n_experts;  // [expert]: where the workgroup's entries of the expert begin
-    uint32_t* scan = base + n_experts;              // one value per thread
+    uint32_t* next = mem;                            // [wave][expert]: where the wave's next entry of the expert goes
+    uint32_t* before = mem + kSortWaves * n_experts; // [expert]: entries of the expert in the workgroups before this one
+    uint32_t* all = before + n_experts;              // [expert]: its entries, then those of all experts before it
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = threadIdx.x; i < kSortWaves * n_experts; i += kSortThreads) next[i] = 0;
+    for (int i = threadIdx.x; i < (kSortWaves + 2) * n_experts; i += kSortThreads) mem[i] = 0;
     __syncthreads();
     const size_t lo = (size_t)blockIdx.x * per_block, hi = lo + per_block < n ? lo + per_block : n;
     const size_t per_wave = (per_block + kSortThreads - 1) / kSortThreads * kWave;
@@ -45,37 +46,59 @@ __global__ __launch_bounds__(kSortThreads) void expert_place_kernel(const uint64
         const uint64_t e = experts[i];
         if (e < (uint64_t)n_experts) atomicAdd(&next[wave * n_experts + e], 1u);
     }
-    __syncthreads();
-    // thread t sums up the experts [t * per, (t + 1) * per): all workgroups' counts, and those of the workgroups before
-    const int per = (n_experts + kSortThreads - 1) / kSortThreads;
-    const int e_lo = threadIdx.x * per, e_hi = e_lo + per < n_experts ? e_lo + per : n_experts;
-    uint32_t mine = 0;
-    for (int e = e_lo; e < e_hi; e++) {
-        uint32_t all = 0, before = 0;
-        if (counts) {
-            for (unsigned b = 0; b < gridDim.x; b++) {
-                const uint32_t c = counts[(size_t)b * n_experts + e];
-                before += b < blockIdx.x ? c : 0u;
-                all += c;
+    if (counts) {
+        // a column of the counts per thread; with fewer experts than threads several threads share one, each with its own runs
+        int wide = kSortThreads;
+        while (wide / 2 >= n_experts) wide /= 2;
+        const unsigned groups = kSortThreads / wide, group = threadIdx.x / wide;
+        for (int e = threadIdx.x % wide; e < n_experts; e += wide) {
+            uint32_t sum = 0, early = 0;
+            for (unsigned b0 = group; b0 < gridDim.x; b0 += 16 * groups) {  // sixteen loads in flight: they come from other XCDs' writes
+                uint32_t c[16];
+#pragma unroll
+                for (int u = 0; u < 16; u++) {
+                    const unsigned b = b0 + u * groups;
+                    c[u] = b < gridDim.x ? counts[(size_t)b * n_experts + e] : 0u;
+                }
+#pragma unroll
+                for (int u = 0; u < 16; u++) {
+                    sum += c[u];
+                    early += b0 + u * groups < blockIdx.x ? c[u] : 0u;
+                }
             }
-        } else {
-            for (int w = 0; w < kSortWaves; w++) all += next[w * n_experts + e];
+            atomicAdd(&all[e], sum);
+            atomicAdd(&before[e], early);
         }
-        base[e] = mine + before;
-        mine += all;
     }
-    scan[threadIdx.x] = mine;
     __syncthreads();
-    for (int d = 1; d < kSortThreads; d <<= 1) {
-        const uint32_t v = (int)threadIdx.x >= d ? scan[threadIdx.x - d] : 0u;
-        __syncthreads();
-        scan[threadIdx.x] += v;
+    if (!counts) {
+        for (int e = threadIdx.x; e < n_experts; e += kSortThreads) {
+            uint32_t c = 0;
+            for (int w = 0; w < kSortWaves; w++) c += next[w * n_experts + e];
+            all[e] = c;
+        }
         __syncthreads();
     }
-    const uint32_t first = scan[threadIdx.x] - mine;  // entries of all experts before this thread's
-    for (int e = e_lo; e < e_hi; e++) {
-        uint32_t at = base[e] + first;
-        base[e] = at;
+    if (wave == 0) {  // exclusive sums over the experts, 64 at a time
+        uint32_t carry = 0;
+        for (int e0 = 0; e0 < n_experts; e0 += kWave) {
+            const int e = e0 + lane;
+            const uint32_t c = e < n_experts ? all[e] : 0u;
+            uint32_t incl = c;
+#pragma unroll
+            for (int d = 1; d < kWave; d <<= 1) {
+                const uint32_t o = (uint32_t)__shfl_up((int)incl, d, kWave);
+                if (lane >= d) incl += o;
+            }
+            if (e < n_experts) all[e] = carry + incl - c;
+            if (blockIdx.x == 0 && e < n_experts) offsets[e] = carry + incl - c;
+            carry += (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1);
+        }
+        if (blockIdx.x == 0 && lane == 0) offsets[n_experts] = carry;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < n_experts; e += kSortThreads) {
+        uint32_t at = all[e] + before[e];
         for (int w = 0; w < kSortWaves; w++) {
             const uint32_t c = next[w * n_experts + e];
             next[w * n_experts + e] = at;
@@ -83,10 +106,6 @@ __global__ __launch_bounds__(kSortThreads) void expert_place_kernel(const uint64
         }
     }
     __syncthreads();
-    if (blockIdx.x == 0) {  // its entries come first, so its bases are the experts' offsets
-        for (int e = threadIdx.x; e < n_experts; e += kSortThreads) offsets[e] = base[e];
-        if (threadIdx.x == kSortThreads - 1) offsets[n_experts] = scan[threadIdx.x];
-    }
     // each wave places its run in order, 64 entries at a time: an entry goes behind the lower lanes of the same expert
     volatile uint32_t* const my_next = next + wave * n_experts;
     for (size_t i0 = w_lo; i0 < w_hi; i0 += kWave) {
@@ -109,71 +128,143 @@ __global__ __launch_bounds__(kSortThreads) void expert_place_kernel(const uint64
 }
 
 // ------------------------------------------------------------------------------------------------
-// rows in the order of their experts, and back
+// Rows in the order of their experts, and back.  All are bound by memory: each row is read and written once, in pieces of four
+// values at whatever 4-byte alignment the rows have (the memory system serves 16-byte accesses there; a row's last piece may
+// hold fewer).  A thread owns a piece of a token's row and walks the token's k entries.
 // ------------------------------------------------------------------------------------------------
-// SCALE: the rows are multiplied by their weights (the backward of the combination)
-template <int V, bool SCALE>
-__global__ __launch_bounds__(kBlock) void expert_spread_kernel(const float* x, const uint64_t* slots, const float* weights,
-                                                                float* y, size_t n_tokens, size_t k, size_t width) {
-    typedef float vec __attribute__((ext_vector_type(V)));
-    const size_t pieces = width / V, total = n_tokens * pieces, places = n_tokens * k;
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ float4u load_piece(const float* row, size_t c, size_t width) {
+    if (c + 4 <= width) return *reinterpret_cast<const float4u*>(row + c);
+    float4u v = {row[c], 0.f, 0.f, 0.f};
+    if (c + 1 < width) v.y = row[c + 1];
+    if (c + 2 < width) v.z = row[c + 2];
+    return v;
+}
+__device__ __forceinline__ void store_piece(float* row, size_t c, size_t width, float4u v) {
+    if (c + 4 <= width) {
+        *reinterpret_cast<float4u*>(row + c) = v;
+        return;
+    }
+    row[c] = v.x;
+    if (c + 1 < width) row[c + 1] = v.y;
+    if (c + 2 < width) row[c + 2] = v.z;
+}
+// Quotient and remainder; a 32-bit division where that does (a 64-bit one costs more than the rest of a piece).
+__device__ __forceinline__ void split(size_t i, size_t by, size_t& q, size_t& rem) {
+    if ((i | by) < ((size_t)1 << 32)) {
+        const uint32_t d = (uint32_t)i / (uint32_t)by;
+        q = d;
+        rem = (uint32_t)i - d * (uint32_t)by;
+    } else {
+        q = i / by;
+        rem = i - q * by;
+    }
+}
+
+constexpr int kEntriesAtOnce = 4;  // of a token, whose loads are in flight together
+
+__global__ __launch_bounds__(kBlock) void expert_spread_kernel(const float* x, const uint64_t* slots, float* y, size_t n_tokens,
+                                                                size_t k, size_t width) {
+    const size_t pieces = (width + 3) / 4, total = n_tokens * pieces, places = n_tokens * k;
     for (size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x; i < total; i += (size_t)gridDim.x * kBlock) {
-        const size_t t = i / pieces, p = i - t * pieces;
-        const vec v = *reinterpret_cast<const vec*>(x + t * width + p * V);
-        for (size_t j = 0; j < k; j++) {
-            const uint64_t s = slots[t * k + j];
-            if (s >= places) continue;
-            vec o = v;
-            if (SCALE) {
-                const float w = weights[t * k + j];
-                for (int u = 0; u < V; u++) o[u] = __fmul_rn(w, v[u]);
-            }
-            *reinterpret_cast<vec*>(y + s * width + p * V) = o;
+        size_t t, p;
+        split(i, pieces, t, p);
+        const float4u v = load_piece(x + t * width, 4 * p, width);
+        for (size_t j0 = 0; j0 < k; j0 += kEntriesAtOnce) {
+            uint64_t s[kEntriesAtOnce];
+#pragma unroll
+            for (int u = 0; u < kEntriesAtOnce; u++) s[u] = j0 + u < k ? slots[t * k + j0 + u] : ~(uint64_t)0;
+#pragma unroll
+            for (int u = 0; u < kEntriesAtOnce; u++)
+                if (s[u] < places) store_piece(y + s[u] * width, 4 * p, width, v);
         }
     }
 }
 
 // SCALE: the weighted sum; else the plain one.  ACC: added to what is there.
-template <int V, bool SCALE, bool ACC>
+template <bool SCALE, bool ACC>
 __global__ __launch_bounds__(kBlock) void expert_gather_kernel(const float* y, const uint64_t* slots, const float* weights,
                                                                 float* out, size_t n_tokens, size_t k, size_t width) {
-    typedef float vec __attribute__((ext_vector_type(V)));
-    const size_t pieces = width / V, total = n_tokens * pieces, places = n_tokens * k;
+    const size_t pieces = (width + 3) / 4, total = n_tokens * pieces, places = n_tokens * k;
     for (size_t i = (size_t)blockIdx.x * kBlock + threadIdx.x; i < total; i += (size_t)gridDim.x * kBlock) {
-        const size_t t = i / pieces, p = i - t * pieces;
-        vec* const to = reinterpret_cast<vec*>(out + t * width + p * V);
-        vec acc;
-        for (int u = 0; u < V; u++) acc[u] = 0.f;
-        if (ACC) acc = *to;
-        for (size_t j = 0; j < k; j++) {
-            const uint64_t s = slots[t * k + j];
-            if (s >= places) continue;
-            const vec v = *reinterpret_cast<const vec*>(y + s * width + p * V);
-            const float w = SCALE ? weights[t * k + j] : 1.f;
-            for (int u = 0; u < V; u++) acc[u] += SCALE ? w * v[u] : v[u];
+        size_t t, p;
+        split(i, pieces, t, p);
+        float4u acc = {0.f, 0.f, 0.f, 0.f};
+        if (ACC) acc = load_piece(out + t * width, 4 * p, width);
+        for (size_t j0 = 0; j0 < k; j0 += kEntriesAtOnce) {
+            bool held[kEntriesAtOnce];
+            float w[kEntriesAtOnce];
+            float4u v[kEntriesAtOnce];
+#pragma unroll
+            for (int u = 0; u < kEntriesAtOnce; u++) {
+                const uint64_t s = j0 + u < k ? slots[t * k + j0 + u] : ~(uint64_t)0;
+                held[u] = s < places;
+                w[u] = SCALE && held[u] ? weights[t * k + j0 + u] : 1.f;
+                v[u] = float4u{0.f, 0.f, 0.f, 0.f};
+                if (held[u]) v[u] = load_piece(y + s * width, 4 * p, width);
+            }
+#pragma unroll
+            for (int u = 0; u < kEntriesAtOnce; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float term = SCALE ? w[u] * v[u][e] : v[u][e];
+                    acc[e] = held[u] ? acc[e] + term : acc[e];
+                }
         }
-        *to = acc;
+        store_piece(out + t * width, 4 * p, width, acc);
     }
 }
 
-// a wave per entry: the product of the row's gradient with the entry's output
-__global__ __launch_bounds__(kBlock) void expert_weight_grad_kernel(const float* out_g, const float* y, const uint64_t* slots,
-                                                                     float* weights_g, size_t n_tokens, size_t k, size_t width) {
-    const int lane = threadIdx.x & 63;
-    const size_t n = n_tokens * k;
-    for (size_t i = (size_t)blockIdx.x * (kBlock / kWave) + (threadIdx.x >> 6); i < n; i += (size_t)gridDim.x * (kBlock / kWave)) {
+// The backward of the combination: L lanes take an entry, scale its token's gradient into its row and sum up the product of that gradient
+// with the entry's output in the same pass.  ROWS / WEIGHTS: which of the two are wanted.
+template <int L, bool ROWS, bool WEIGHTS>
+__global__ __launch_bounds__(kBlock) void expert_combine_bwd_kernel(const float* out_g, const float* y, const uint64_t* slots,
+                                                                     const float* weights, float* y_g, float* weights_g,
+                                                                     size_t n_tokens, size_t k, size_t width) {
+    constexpr int U = 4;
+    const int lane = threadIdx.x % L;
+    const size_t n = n_tokens * k, pieces = (width + 3) / 4;
+    for (size_t i = (size_t)blockIdx.x * (kBlock / L) + threadIdx.x / L; i < n; i += (size_t)gridDim.x * (kBlock / L)) {
         const uint64_t s = slots[i];
         float sum = 0.f;
-        if (s < n)
-            for (size_t c = lane; c < width; c += kWave) sum += out_g[i / k * width + c] * y[s * width + c];
-        sum = group_reduce<SumAcc>(sum);
-        if (lane == 0) weights_g[i] = sum;
+        if (s < n) {
+            size_t t, j;
+            split(i, k, t, j);
+            const float w = ROWS ? weights[i] : 0.f;
+            const float* g_row = out_g + t * width;
+            const float* y_row = WEIGHTS ? y + s * width : nullptr;
+            for (size_t p0 = lane; p0 < pieces; p0 += U * L) {
+                float4u g[U], v[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const size_t p = p0 + (size_t)u * L;
+                    g[u] = v[u] = float4u{0.f, 0.f, 0.f, 0.f};
+                    if (p < pieces) {
+                        g[u] = load_piece(g_row, 4 * p, width);
+                        if (WEIGHTS) v[u] = load_piece(y_row, 4 * p, width);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const size_t p = p0 + (size_t)u * L;
+                    if (WEIGHTS) sum += (g[u].x * v[u].x + g[u].y * v[u].y) + (g[u].z * v[u].z + g[u].w * v[u].w);
+                    if (ROWS && p < pieces)
+                        store_piece(y_g + s * width, 4 * p, width, float4u{w * g[u].x, w * g[u].y, w * g[u].z, w * g[u].w});
+                }
+            }
+        }
+        if (WEIGHTS) {
+#pragma unroll
+            for (int m = L / 2; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, kWave);
+            if (lane == 0) weights_g[i] = sum;
+        }
     }
 }
 
 static unsigned flat_grid(size_t items) {
     const size_t b = ceil_div_sz(items, kBlock);
-    return (unsigned)(b < 65536 ? b : 65536);
+    return (unsigned)(b < 1048576 ? b : 1048576);
 }
 static int experts_check(const char* op, const uint64_t* slots, size_t n_tokens, size_t k, size_t width) {
     ZG_REQUIRE(k >= 1 && k <= ZG_HIP_EXPERTS_MAX_K, "%s: k = %zu is not in 1 .. %d", op, k, (int)ZG_HIP_EXPERTS_MAX_K);
@@ -199,8 +290,10 @@ ZG_API int zg_hip_expert_sort(zg_hip_ctx* ctx, const uint64_t* experts, uint64_t
                    !ranges_overlap(slots, n_entries * 8, offsets, (n_experts + 1) * 8),
                "expert_sort: two arrays overlap");
     DeviceGuard guard(ctx);
+    // runs of 1024 entries or more; every workgroup reads all runs' counts, so many experts get fewer runs
+    const size_t most = n_experts < 128 ? 256 : 32768 / n_experts;
     size_t blocks = n_entries <= kSortAlone ? 1 : ceil_div_sz(n_entries, 1024);
-    if (blocks > kSortMaxBlocks) blocks = kSortMaxBlocks;
+    if (blocks > most) blocks = most;
     const size_t per_block = ceil_div_sz(ceil_div_sz(n_entries, blocks), kSortThreads) * kSortThreads;
     blocks = n_entries ? ceil_div_sz(n_entries, per_block) : 1;
     uint32_t* counts = nullptr;
@@ -211,7 +304,7 @@ ZG_API int zg_hip_expert_sort(zg_hip_ctx* ctx, const uint64_t* experts, uint64_t
                            n_entries, per_block, (int)n_experts);
         ZG_LAUNCH_CHECK();
     }
-    const size_t lds = ((kSortWaves + 1) * n_experts + kSortThreads) * sizeof(uint32_t);
+    const size_t lds = (kSortWaves + 2) * n_experts * sizeof(uint32_t);
     hipLaunchKernelGGL(expert_place_kernel, dim3((unsigned)blocks), dim3(kSortThreads), lds, ctx->stream, experts, counts, offsets,
                        slots, n_entries, per_block, (int)n_experts);
     ZG_LAUNCH_CHECK();
@@ -228,11 +321,8 @@ ZG_API int zg_hip_expert_dispatch(zg_hip_ctx* ctx, const float* x, const uint64_
     ZG_REQUIRE(!ranges_overlap(y, bytes, x, n_tokens * width * 4) && !ranges_overlap(y, bytes, slots, n_tokens * k * 8),
                "expert_dispatch: y overlaps an input");
     DeviceGuard guard(ctx);
-    const bool vec = width % 4 == 0 && aligned16(x) && aligned16(y);
-    if (vec) hipLaunchKernelGGL((expert_spread_kernel<4, false>), dim3(flat_grid(n_tokens * (width / 4))), dim3(kBlock), 0, ctx->stream,
-                                x, slots, (const float*)nullptr, y, n_tokens, k, width);
-    else hipLaunchKernelGGL((expert_spread_kernel<1, false>), dim3(flat_grid(n_tokens * width)), dim3(kBlock), 0, ctx->stream, x, slots,
-                            (const float*)nullptr, y, n_tokens, k, width);
+    hipLaunchKernelGGL(expert_spread_kernel, dim3(flat_grid(n_tokens * ((width + 3) / 4))), dim3(kBlock), 0, ctx->stream, x, slots, y,
+                       n_tokens, k, width);
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
 }
@@ -241,11 +331,8 @@ namespace zg {
 template <bool SCALE, bool ACC>
 static int launch_gather(zg_hip_ctx* ctx, const float* y, const uint64_t* slots, const float* weights, float* out, size_t n_tokens,
                          size_t k, size_t width) {
-    const bool vec = width % 4 == 0 && aligned16(y) && aligned16(out);
-    if (vec) hipLaunchKernelGGL((expert_gather_kernel<4, SCALE, ACC>), dim3(flat_grid(n_tokens * (width / 4))), dim3(kBlock), 0,
-                                ctx->stream, y, slots, weights, out, n_tokens, k, width);
-    else hipLaunchKernelGGL((expert_gather_kernel<1, SCALE, ACC>), dim3(flat_grid(n_tokens * width)), dim3(kBlock), 0, ctx->stream, y,
-                            slots, weights, out, n_tokens, k, width);
+    hipLaunchKernelGGL((expert_gather_kernel<SCALE, ACC>), dim3(flat_grid(n_tokens * ((width + 3) / 4))), dim3(kBlock), 0, ctx->stream, y,
+                       slots, weights, out, n_tokens, k, width);
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
 }
@@ -294,18 +381,21 @@ ZG_API int zg_hip_expert_combine_bwd(zg_hip_ctx* ctx, const float* out_g, const 
                    !ranges_overlap(weights_g, n * 4, slots, n * 8) && !ranges_overlap(weights_g, n * 4, weights, n * 4),
                "expert_combine_bwd: weights_g overlaps another operand");
     DeviceGuard guard(ctx);
-    if (y_g) {
-        const bool vec = width % 4 == 0 && aligned16(out_g) && aligned16(y_g);
-        if (vec) hipLaunchKernelGGL((expert_spread_kernel<4, true>), dim3(flat_grid(n_tokens * (width / 4))), dim3(kBlock), 0,
-                                    ctx->stream, out_g, slots, weights, y_g, n_tokens, k, width);
-        else hipLaunchKernelGGL((expert_spread_kernel<1, true>), dim3(flat_grid(n_tokens * width)), dim3(kBlock), 0, ctx->stream, out_g,
-                                slots, weights, y_g, n_tokens, k, width);
-        ZG_LAUNCH_CHECK();
+    if (!y_g && !weights_g) return ZG_HIP_OK;
+    // 16 lanes an entry for narrow rows, a wave else
+#define ZG_COMBINE_BWD(L, ROWS, WEIGHTS)                                                                                            \
+    hipLaunchKernelGGL((expert_combine_bwd_kernel<L, ROWS, WEIGHTS>), dim3(flat_grid(n * (L))), dim3(kBlock), 0, ctx->stream, out_g, y, \
+                       slots, weights, y_g, weights_g, n_tokens, k, width)
+    if (width <= 128) {
+        if (y_g && weights_g) ZG_COMBINE_BWD(16, true, true);
+        else if (y_g) ZG_COMBINE_BWD(16, true, false);
+        else ZG_COMBINE_BWD(16, false, true);
+    } else {
+        if (y_g && weights_g) ZG_COMBINE_BWD(64, true, true);
+        else if (y_g) ZG_COMBINE_BWD(64, true, false);
+        else ZG_COMBINE_BWD(64, false, true);
     }
-    if (weights_g) {
-        hipLaunchKernelGGL(expert_weight_grad_kernel, dim3(flat_grid(n * kWave)), dim3(kBlock), 0, ctx->stream, out_g, y, slots,
-                           weights_g, n_tokens, k, width);
-        ZG_LAUNCH_CHECK();
-    }
+#undef ZG_COMBINE_BWD
+    ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
 }
