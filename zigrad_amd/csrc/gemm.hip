@@ -224,6 +224,7 @@ struct GemmArgs {
     int relu;
     // Experts' products (kernels with GROUP != 0): expert e's rows are offsets[e] .. offsets[e + 1] - 1 of n_rows
     const uint64_t* offsets;
+    const uint32_t* order;  // the experts, those with most rows first (null with at most 64: the workgroups find out themselves)
     unsigned n_experts;
     size_t n_rows;
 };
@@ -275,6 +276,22 @@ __device__ __forceinline__ ExpertTile find_expert_tile(const uint64_t* offsets, 
         before = (unsigned)__builtin_amdgcn_readlane((int)incl, kWave - 1);
     }
     return {0, 0, 0, 0};  // not reached: the caller has checked tile_m against expert_tiles()
+}
+
+// The expert with the n-th most rows of at most 64 (the lower one first among equals) and its rows.  Every wave finds it by itself.
+__device__ __forceinline__ unsigned nth_longest(const uint64_t* offsets, unsigned n_experts, size_t n_rows, unsigned n, int lane,
+                                                uint32_t& first, uint32_t& count) {
+    uint32_t f = 0, c = 0;
+    if ((unsigned)lane < n_experts) expert_range(offsets, lane, n_rows, f, c);
+    unsigned rank = 0;
+    for (int e = 0; e < (int)n_experts; e++) {
+        const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)c, e);
+        rank += o > c || (o == c && e < lane) ? 1u : 0u;
+    }
+    const int l = __builtin_ctzll(__ballot((unsigned)lane < n_experts && rank == n));
+    first = (uint32_t)__builtin_amdgcn_readlane((int)f, l);
+    count = (uint32_t)__builtin_amdgcn_readlane((int)c, l);
+    return (unsigned)l;
 }
 
 // the epilogue extras on one value (the rounding of the separate add / relu / mask kernels: one IEEE add, selects)
@@ -370,7 +387,13 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_kernel(GemmArgs g) {
         z = 0;
     } else if constexpr (GROUP == 2) {
         uint32_t first, count;
-        expert_range(g.offsets, blockIdx.z, g.n_rows, first, count);
+        if (g.order) {
+            z = g.order[blockIdx.z];
+            expert_range(g.offsets, (unsigned)z, g.n_rows, first, count);
+        } else {
+            z = nth_longest(g.offsets, g.n_experts, g.n_rows, blockIdx.z, threadIdx.x & 63, first, count);
+        }
+        z = (size_t)(unsigned)__builtin_amdgcn_readfirstlane((int)z);
         first = (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
         count = (uint32_t)__builtin_amdgcn_readfirstlane((int)count);
         tile_coords(xcd_contiguous(blockIdx.x, g.tiles_m * g.tiles_n), g.tiles_m, g.tiles_n, tm, tn);
@@ -1517,6 +1540,7 @@ static GemmArgs gemm_args(const float* A, const float* B, float* C, size_t m, si
     g.c_vec = 0;
     g.bounded_tail = 0;
     g.offsets = nullptr;
+    g.order = nullptr;
     g.n_experts = 0;
     g.n_rows = 0;
     return g;
@@ -2575,7 +2599,132 @@ static int expert_linear_check(const char* op, const uint64_t* offsets, size_t n
     return ZG_HIP_OK;
 }
 
-// C[rows of e] = A[rows of e] op(B_e) with the extras
+// A few rows per expert: what counts is reading the weights, so a workgroup takes 16 RB rows of one expert by 16 CB columns and asks for
+// all it needs of both at once: each of its four waves reads a run of k, BATCH chunks of 16 values at a time in flight, straight
+// into the operand registers (lane (r, q) holds the values k = 4 q .. 4 q + 3 of a chunk for row r of A and column r of B; the
+// c-th of them feed the chunk's c-th MFMA; a B that is not k-contiguous is read value by value, 16 columns a lane group).  The waves'
+// blocks are added in order.
+template <int RB, int CB, int BATCH, bool B_KMAJOR>
+__global__ __launch_bounds__(256) void expert_few_kernel(GemmArgs g) {
+    __shared__ float part[4][RB * CB][64][4];
+    typedef float piece4 __attribute__((ext_vector_type(4), aligned(4)));
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int r = lane & 15, q = lane >> 4;
+    const unsigned tile_m = blockIdx.x / g.tiles_n, tn = blockIdx.x % g.tiles_n;
+    if (tile_m >= expert_tiles<16 * RB>(g.offsets, g.n_experts, g.n_rows, lane)) return;
+    const ExpertTile t = find_expert_tile<16 * RB>(g.offsets, g.n_experts, g.n_rows, tile_m, lane);
+    const unsigned left = t.count - t.tile * 16 * RB, rows = left < 16 * RB ? left : 16 * RB;  // of this tile
+    const size_t first = (size_t)t.first + t.tile * 16 * RB, col0 = (size_t)tn * 16 * CB;
+    const unsigned cols = g.N - col0 < 16 * CB ? (unsigned)(g.N - col0) : 16u * CB;
+    // rows and columns past the edge repeat the last one; their sums are never stored
+    const float *a[RB], *b[CB];
+#pragma unroll
+    for (int i = 0; i < RB; i++) a[i] = g.A + (first + (16u * i + r < rows ? 16u * i + r : rows - 1)) * g.lda + 4 * q;
+#pragma unroll
+    for (int j = 0; j < CB; j++) {
+        const size_t col = col0 + (16u * j + r < cols ? 16u * j + r : cols - 1);
+        b[j] = g.B + (size_t)t.e * g.b_chunk + (B_KMAJOR ? col * g.ldb + 4 * q : 4 * q * g.ldb + col);
+    }
+    // four values of k of a whole chunk
+    auto load_a = [&](int i, size_t chunk) { return *reinterpret_cast<const piece4*>(a[i] + chunk * 16); };
+    auto load_b = [&](int j, size_t chunk) {
+        if (B_KMAJOR) return *reinterpret_cast<const piece4*>(b[j] + chunk * 16);
+        piece4 v;
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[c] = b[j][(chunk * 16 + c) * g.ldb];
+        return v;
+    };
+    const unsigned chunks = (unsigned)((g.K + 15) / 16), whole = (unsigned)(g.K / 16);
+    const unsigned per_wave = (chunks + 3) / 4;
+    const unsigned lo = wave * per_wave, hi = lo + per_wave < chunks ? lo + per_wave : chunks;
+    const unsigned full = hi < whole ? hi : whole;
+    floatx4 acc[RB][CB];
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+        for (int j = 0; j < CB; j++) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const piece4 (&av)[RB], const piece4 (&bv)[CB]) {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < RB; i++)
+#pragma unroll
+                for (int j = 0; j < CB; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[i][c], bv[j][c], acc[i][j], 0, 0, 0);
+    };
+    unsigned c0 = lo;
+    for (; c0 + BATCH <= full; c0 += BATCH) {
+        piece4 av[BATCH][RB], bv[BATCH][CB];
+#pragma unroll
+        for (int s = 0; s < BATCH; s++) {
+#pragma unroll
+            for (int j = 0; j < CB; j++) bv[s][j] = load_b(j, c0 + s);
+#pragma unroll
+            for (int i = 0; i < RB; i++) av[s][i] = load_a(i, c0 + s);
+        }
+#pragma unroll
+        for (int s = 0; s < BATCH; s++) multiply(av[s], bv[s]);
+    }
+    for (; c0 < hi; c0++) {  // what is left of the run, the chunk that k ends in value by value
+        piece4 av[RB], bv[CB];
+#pragma unroll
+        for (int i = 0; i < RB; i++) {
+            if (c0 < whole) {
+                av[i] = load_a(i, c0);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; c++) av[i][c] = (size_t)c0 * 16 + 4 * q + c < g.K ? a[i][(size_t)c0 * 16 + c] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < CB; j++) {
+            if (c0 < whole) {
+                bv[j] = load_b(j, c0);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const size_t k = (size_t)c0 * 16 + c;
+                    bv[j][c] = k + 4 * q < g.K ? b[j][B_KMAJOR ? k : k * g.ldb] : 0.f;
+                }
+            }
+        }
+        multiply(av, bv);
+    }
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+        for (int j = 0; j < CB; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) part[wave][i * CB + j][lane][e] = acc[i][j][e];
+    __syncthreads();
+    // accumulator e of lane (r, q) is the block's element (4 q + e, r)
+    const unsigned er = threadIdx.x >> 4, ec = threadIdx.x & 15;
+    const int src_lane = (er >> 2) * 16 + ec, src_e = er & 3;
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+        for (int j = 0; j < CB; j++) {
+            float sum = part[0][i * CB + j][src_lane][src_e];
+#pragma unroll
+            for (int w = 1; w < 4; w++) sum += part[w][i * CB + j][src_lane][src_e];
+            const unsigned row = 16 * i + er, col = 16 * j + ec;
+            if (row >= rows || col >= cols) continue;
+            const float bias = g.bias ? g.bias[(size_t)t.e * g.N + col0 + col] : 0.f;
+            const size_t at = (first + row) * g.ldc + col0 + col;
+            const float v = gemm_extras(sum, g.bias != nullptr, bias, g.relu != 0);
+            g.C[at] = g.gate && g.gate[at] <= 0.f ? 0.f : v;
+        }
+}
+template <int RB, int CB, int BATCH, bool B_KMAJOR>
+static int launch_expert_few(zg_hip_ctx* ctx, GemmArgs g) {
+    g.tiles_n = (unsigned)ceil_div_sz(g.N, 16 * CB);
+    const size_t most = g.n_rows / (16 * RB) + (g.n_rows < g.n_experts ? g.n_rows : g.n_experts);
+    ZG_REQUIRE(most * g.tiles_n < 0x7fffffffull, "expert_linear: %zu workgroups", most * g.tiles_n);
+    hipLaunchKernelGGL((expert_few_kernel<RB, CB, BATCH, B_KMAJOR>), dim3((unsigned)(most * g.tiles_n)), dim3(256), 0, ctx->stream, g);
+    ZG_LAUNCH_CHECK();
+    return ZG_HIP_OK;
+}
+
+// C[rows of e] = A[rows of e] op(B_e) with the extras, tile by tile
 template <int BM, int BN, bool B_KMAJOR>
 static int launch_expert_rows(zg_hip_ctx* ctx, GemmArgs g) {
     g.tiles_n = (unsigned)ceil_div_sz(g.N, BN);
@@ -2599,6 +2748,23 @@ static int expert_rows(zg_hip_ctx* ctx, const float* A, const float* B, float* C
     g.split_tiles = ceil_div_sz(k, kBK);
     g.c_vec = aligned16(C) && n % 4 == 0 && (!gate || aligned16(gate));
     g.bounded_tail = !B_KMAJOR && n % 4 != 0;
+    // Few rows per expert: the kernel above, with 16 x 16 or 32 x 32 blocks, as long as it reads the weights once or twice only or the
+    // staged kernel's 64 x 64 tiles do not fill the compute units (measured at 8 to 64 experts of 300 x 500 to 4096 x 4096).
+    // k-contiguous weights (forward), 1024 -> 2048, 8 experts: 32 rows 11 against 21 us, 256 rows 29 against 35, 512 rows 39
+    // against 36; 1024 -> 1024, 64 experts: 1024 rows 56 against 64, 2048 rows 84 against 65.
+    // Weights read value by value (input gradient), the same layers: 32 rows 17 against 42 us, 256 rows 31 against 43; 64 experts:
+    // 64 rows 33 against 44, 256 rows 59 against 51.
+    const size_t per = n_rows / n_experts, n_cu = (size_t)ctx->n_cu;
+    const size_t tiles = (n_rows / 64 + (n_rows < n_experts ? n_rows : n_experts)) * ceil_div_sz(n, 64);
+    if (B_KMAJOR) {
+        if (per <= 6) return launch_expert_few<1, 1, 8, B_KMAJOR>(ctx, g);
+        if (per <= 20 || (per <= 48 && tiles <= n_cu)) return launch_expert_few<2, 2, 4, B_KMAJOR>(ctx, g);
+    } else {
+        if (per <= 2 || (per <= 16 && tiles <= n_cu)) return launch_expert_few<1, 1, 8, B_KMAJOR>(ctx, g);
+        if (per <= 32 && tiles <= 3 * n_cu) return launch_expert_few<2, 2, 4, B_KMAJOR>(ctx, g);
+    }
+    // 64 x 64 tiles: the larger ones waste more on the last tile of every expert than they gain (16384 rows, 16 experts, 1024 -> 2048:
+    // 536 us, 128 x 128 533, 256 x 128 595; 64 experts, 1024 -> 1024: 308, 356 and 473 us)
     return launch_expert_rows<64, 64, B_KMAJOR>(ctx, g);
 }
 // C_e (+)= A[rows of e]^T B[rows of e]
@@ -2614,25 +2780,160 @@ static int launch_expert_weights(zg_hip_ctx* ctx, GemmArgs g) {
     return ZG_HIP_OK;
 }
 
-// gb_e (+)= column sums of expert e's rows: 64 columns x 4 row-threads
+// Weight gradients of experts with few rows, bound by writing them: a thread owns a piece of four inputs and OUTS outputs and walks the
+// expert's rows, its x pieces in flight eight at a time, gy by scalar loads.  tx threads side by side along the inputs, 256 / tx
+// groups of outputs.  (64 experts of 1024 x 1024, one of them with 42 of 256
+// rows: 40 us, 6.9 TB/s; the staged kernel with its 4-byte stores 97 us.)
+constexpr int kFewOuts = 8;
 template <bool ACC>
-__global__ __launch_bounds__(256) void expert_bias_grad_kernel(const float* gy, float* gb, const uint64_t* offsets, size_t n_rows,
+__global__ __launch_bounds__(256, 4) void expert_weights_few_kernel(const float* gy, const float* x, float* gw, const uint64_t* offsets,
+                                                                  size_t n_rows, size_t fan_in, size_t fan_out, int tx) {
+    typedef float piece __attribute__((ext_vector_type(4), aligned(4)));
+    uint32_t first, count;
+    expert_range(offsets, blockIdx.z, n_rows, first, count);
+    first = (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
+    count = (uint32_t)__builtin_amdgcn_readfirstlane((int)count);
+    const size_t c = ((size_t)blockIdx.x * tx + threadIdx.x % tx) * 4;
+    // a wave's threads share their outputs (tx is a multiple of 64), so what they read of gy is the same for all
+    const size_t o0 = ((size_t)blockIdx.y * (256 / tx) + (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / tx))) * kFewOuts;
+    if (c >= fan_in || o0 >= fan_out) return;
+    const int outs = fan_out - o0 < kFewOuts ? (int)(fan_out - o0) : kFewOuts;
+    const bool whole = c + 4 <= fan_in;
+    piece acc[kFewOuts];
+#pragma unroll
+    for (int o = 0; o < kFewOuts; o++) acc[o] = piece{0.f, 0.f, 0.f, 0.f};
+    constexpr int R = 8;
+    for (uint32_t r0 = 0; r0 < count; r0 += R) {
+        piece v[R];
+#pragma unroll
+        for (int u = 0; u < R; u++) {
+            v[u] = piece{0.f, 0.f, 0.f, 0.f};
+            if (r0 + u < count) {
+                const float* p = x + (size_t)(first + r0 + u) * fan_in + c;
+                if (whole) {
+                    v[u] = *reinterpret_cast<const piece*>(p);
+                } else {
+                    v[u].x = p[0];
+                    if (c + 1 < fan_in) v[u].y = p[1];
+                    if (c + 2 < fan_in) v[u].z = p[2];
+                }
+            }
+        }
+        const float* g = gy + (size_t)(first + r0) * fan_out + o0;
+        if (outs == kFewOuts && r0 + R <= count) {  // adjacent values of gy by one scalar load a row, all rows' under way together
+            float a[R][kFewOuts];
+#pragma unroll
+            for (int u = 0; u < R; u++)
+#pragma unroll
+                for (int o = 0; o < kFewOuts; o++) a[u][o] = g[u * fan_out + o];
+#pragma unroll
+            for (int u = 0; u < R; u++)
+#pragma unroll
+                for (int o = 0; o < kFewOuts; o++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[o][e] = __builtin_fmaf(a[u][o], v[u][e], acc[o][e]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < R; u++) {
+                if (r0 + u >= count) break;
+#pragma unroll
+                for (int o = 0; o < kFewOuts; o++) {
+                    const float a = o < outs ? g[u * fan_out + o] : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[o][e] = __builtin_fmaf(a, v[u][e], acc[o][e]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 0; o < kFewOuts; o++) {
+        if (o >= outs) break;
+        float* to = gw + ((size_t)blockIdx.z * fan_out + o0 + o) * fan_in + c;
+        if (whole) {
+            piece s = acc[o];
+            if (ACC) s = *reinterpret_cast<const piece*>(to) + s;
+            *reinterpret_cast<piece*>(to) = s;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+                if (c + e < fan_in) to[e] = ACC ? to[e] + acc[o][e] : acc[o][e];
+        }
+    }
+}
+
+// The experts by their number of rows, most first: a thread counts how many come before its own.
+__global__ __launch_bounds__(1024) void expert_order_kernel(const uint64_t* offsets, uint32_t* order, unsigned n_experts, size_t n_rows) {
+    __shared__ uint32_t counts[ZG_HIP_EXPERTS_MAX];
+    const unsigned e = threadIdx.x;
+    uint32_t first, mine = 0;
+    if (e < n_experts) {
+        expert_range(offsets, e, n_rows, first, mine);
+        counts[e] = mine;
+    }
+    __syncthreads();
+    if (e >= n_experts) return;
+    unsigned rank = 0;
+#pragma unroll 8
+    for (unsigned o = 0; o < n_experts; o++) rank += counts[o] > mine || (counts[o] == mine && o < e) ? 1u : 0u;
+    order[rank] = e;
+}
+
+// Column sums of the experts' rows: 32 lanes of four columns by 8 row-threads with eight rows in flight.  Each expert's rows are cut
+// into gridDim.z parts, so that one expert with most of the rows does not hold up the rest; a part's sums go to `out` (laid out
+// [part][expert][column]), which expert_bias_join_kernel adds up in order, or, with a single part, to the gradient itself.
+template <bool ACC>
+__global__ __launch_bounds__(256) void expert_bias_grad_kernel(const float* gy, float* out, const uint64_t* offsets, size_t n_rows,
                                                                 size_t fan_out) {
-    __shared__ float part[4][64];
+    __shared__ float4 part[8][32];
     uint32_t first, count;
     expert_range(offsets, blockIdx.y, n_rows, first, count);
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const size_t col = (size_t)blockIdx.x * 64 + tx;
-    float sum = 0.f;
-    if (col < fan_out)
-        for (uint32_t r = ty; r < count; r += 4) sum += gy[(size_t)(first + r) * fan_out + col];
-    part[ty][tx] = sum;
-    __syncthreads();
-    if (ty == 0 && col < fan_out) {
-        float* to = gb + (size_t)blockIdx.y * fan_out + col;
-        const float v = (part[0][tx] + part[1][tx]) + (part[2][tx] + part[3][tx]);
-        *to = ACC ? *to + v : v;
+    const uint32_t lo = (uint32_t)((uint64_t)count * blockIdx.z / gridDim.z), hi = (uint32_t)((uint64_t)count * (blockIdx.z + 1) / gridDim.z);
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+    const size_t col = (size_t)blockIdx.x * 128 + 4 * tx;
+    typedef float piece __attribute__((ext_vector_type(4), aligned(4)));
+    const size_t have = col < fan_out ? fan_out - col : 0;  // columns of this thread, if fewer than four
+    piece sum = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t r0 = lo + ty; r0 < hi; r0 += 64) {
+        piece v[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const uint32_t r = r0 + 8 * u;
+            v[u] = piece{0.f, 0.f, 0.f, 0.f};
+            if (r < hi) {
+                const float* p = gy + (size_t)(first + r) * fan_out + col;
+                if (have >= 4) {
+                    v[u] = *reinterpret_cast<const piece*>(p);
+                } else {
+                    if (have > 0) v[u].x = p[0];
+                    if (have > 1) v[u].y = p[1];
+                    if (have > 2) v[u].z = p[2];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] += v[u][e];
     }
+    part[ty][tx] = make_float4(sum.x, sum.y, sum.z, sum.w);
+    __syncthreads();
+    if (ty != 0) return;
+    float* to = out + ((size_t)blockIdx.z * gridDim.y + blockIdx.y) * fan_out + col;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if ((size_t)e >= have) break;
+        float s = 0.f;
+#pragma unroll
+        for (int y = 0; y < 8; y++) s += reinterpret_cast<const float*>(&part[y][tx])[e];
+        to[e] = ACC ? to[e] + s : s;
+    }
+}
+__global__ __launch_bounds__(256) void expert_bias_join_kernel(const float* parts, float* gb, size_t n, unsigned n_parts, int accumulate) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float s = 0.f;
+    for (unsigned p = 0; p < n_parts; p++) s += parts[(size_t)p * n + i];
+    gb[i] = accumulate ? gb[i] + s : s;
 }
 }  // namespace zg
 
@@ -2680,12 +2981,55 @@ ZG_API int zg_hip_expert_linear_bwd(zg_hip_ctx* ctx, const float* gy, const floa
     g.split_tiles = (size_t)1 << 28;  // all of k
     g.c_vec = aligned16(gw) && fan_in % 4 == 0;
     g.bounded_tail = fan_out % 4 != 0 || fan_in % 4 != 0;
-    if (int rc = launch_expert_weights<64, 64>(ctx, g)) return rc;
-    if (gb) {
-        const dim3 grid((unsigned)ceil_div_sz(fan_out, 64), (unsigned)n_experts);
-        if (accumulate) hipLaunchKernelGGL(expert_bias_grad_kernel<true>, grid, dim3(256), 0, ctx->stream, gy, gb, offsets, n_rows, fan_out);
-        else hipLaunchKernelGGL(expert_bias_grad_kernel<false>, grid, dim3(256), 0, ctx->stream, gy, gb, offsets, n_rows, fan_out);
+    // few rows: the kernel that writes wide (64 experts of 512 x 512, 512 rows: 28 against 32 us, 1024 rows: 44 against 34)
+    const bool few = n_rows / n_experts <= 8;
+    // workspace: the experts' order, then the parts of the bias gradient
+    const size_t order_bytes = n_experts > kWave && !few ? (n_experts * sizeof(uint32_t) + 255) / 256 * 256 : 0;
+    size_t parts = 1;  // about 128 rows of an average expert each
+    if (gb) parts = n_rows / (n_experts * 128);
+    if (parts > 16) parts = 16;
+    if (parts < 1) parts = 1;
+    const size_t need = order_bytes + (gb && parts > 1 ? parts * n_experts * fan_out * sizeof(float) : 0);
+    char* ws = nullptr;
+    if (need) {
+        ws = (char*)workspace(ctx, need);
+        if (!ws) return ZG_HIP_EOOM;
+    }
+    if (few) {
+        int tx = 64;
+        while (tx < 256 && (size_t)tx * 4 < fan_in) tx *= 2;
+        const dim3 grid((unsigned)ceil_div_sz(fan_in, 4 * tx), (unsigned)ceil_div_sz(fan_out, 256 / tx * kFewOuts), (unsigned)n_experts);
+        ZG_REQUIRE(grid.y < 65536, "expert_linear_bwd: %zu outputs", fan_out);
+        if (accumulate)
+            hipLaunchKernelGGL(expert_weights_few_kernel<true>, grid, dim3(256), 0, ctx->stream, gy, x, gw, offsets, n_rows, fan_in, fan_out, tx);
+        else
+            hipLaunchKernelGGL(expert_weights_few_kernel<false>, grid, dim3(256), 0, ctx->stream, gy, x, gw, offsets, n_rows, fan_in, fan_out, tx);
         ZG_LAUNCH_CHECK();
+    } else {
+        if (order_bytes) {
+            hipLaunchKernelGGL(expert_order_kernel, dim3(1), dim3(1024), 0, ctx->stream, offsets, (uint32_t*)ws, (unsigned)n_experts, n_rows);
+            ZG_LAUNCH_CHECK();
+            g.order = (const uint32_t*)ws;
+        }
+        // 128 x 128 tiles where there are several for every compute unit (16 experts of 2048 x 1024, 16384 rows: 490 us against 548 with
+        // 64 x 64), else the smaller ones (64 experts of 512 x 512, 4096 rows, one expert with 609: 88 us the three products against 96)
+        const bool large = n_experts * ceil_div_sz(fan_out, 128) * ceil_div_sz(fan_in, 128) >= 6 * (size_t)ctx->n_cu;
+        if (int rc = large ? launch_expert_weights<128, 128>(ctx, g) : launch_expert_weights<64, 64>(ctx, g)) return rc;
+    }
+    if (gb) {
+        const dim3 grid((unsigned)ceil_div_sz(fan_out, 128), (unsigned)n_experts, (unsigned)parts);
+        float* out = parts > 1 ? (float*)(ws + order_bytes) : gb;
+        if (parts == 1 && accumulate)
+            hipLaunchKernelGGL(expert_bias_grad_kernel<true>, grid, dim3(256), 0, ctx->stream, gy, out, offsets, n_rows, fan_out);
+        else
+            hipLaunchKernelGGL(expert_bias_grad_kernel<false>, grid, dim3(256), 0, ctx->stream, gy, out, offsets, n_rows, fan_out);
+        ZG_LAUNCH_CHECK();
+        if (parts > 1) {
+            const size_t n = n_experts * fan_out;
+            hipLaunchKernelGGL(expert_bias_join_kernel, dim3((unsigned)ceil_div_sz(n, 256)), dim3(256), 0, ctx->stream, out, gb, n,
+                               (unsigned)parts, accumulate ? 1 : 0);
+            ZG_LAUNCH_CHECK();
+        }
     }
     if (!gx || n_rows == 0) return ZG_HIP_OK;
     return expert_rows<false>(ctx, gy, w, gx, offsets, n_rows, n_experts, fan_in, fan_out, nullptr, act_in, 0);
