@@ -726,7 +726,7 @@ __global__ __launch_bounds__(256) void topk_bwd_add_kernel(const uint64_t* indic
 //   e_c = 2^((x_c - m) c), s = sum e_c, p_c = e_c / s      f_j = 2^((t_j - tm) c), S = sum f_j, q_j = f_j / S
 //   row_loss = T^2 (sum_j f_j ((t_j - tm) - (x_{i_j} - m)) / T / S - log S + log s)
 // A row's logits are read once, into registers, by 16 lanes, a wave, or a workgroup of 256 or 1024, by its length (rows of
-// more than 65536 columns are read twice); the maxima, then all sums, take one reduction each.  For the gradient the q_j go into a
+// more than 65536 columns are read twice for the gradient); the maxima, then all sums, take one reduction each.  For the gradient the q_j go into a
 // stretch of LDS laid out like the row, from where every thread takes what belongs to its columns: the gradient leaves in whole
 // 16-byte pieces, written once, and a class that is named twice gets both shares, added in the order of j by one wave.
 // ------------------------------------------------------------------------------------------------
@@ -980,11 +980,15 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 && VPT == 8 && !ACC
     float* const span = span_mem + (BWD ? sub * kSpan : 0);
     uint32_t* const col_of = col_mem + (BWD ? sub * kMaxK : 0);
     float* const q_of = q_mem + (BWD ? sub * kMaxK : 0);
-    const size_t r = (size_t)blockIdx.x * kRows + sub;
+    // The gradient alone, whose statistics are known, is done segment by segment of a long row (first, cols: this one's columns).
+    const size_t job = (size_t)blockIdx.x * kRows + sub;
+    const uint32_t segments = FWD ? 1u : (a.cols - 1) / (4 * NT * VPT) + 1;
+    const size_t r = FWD ? job : job / segments;
     if (r >= a.rows) return;  // only waves that own a row of their own: no barrier is missed
-    const uint32_t cols = a.cols, whole = cols & ~3u;
-    const float* x = a.x + r * cols;
-    float* grad = BWD ? a.grad + r * cols : nullptr;
+    const uint32_t first = FWD ? 0u : (uint32_t)(job - r * segments) * (4 * NT * VPT);
+    const uint32_t cols = FWD || a.cols - first < 4 * NT * VPT ? a.cols - first : 4 * NT * VPT, whole = cols & ~3u;
+    const float* x = a.x + r * a.cols + first;
+    float* grad = BWD ? a.grad + r * a.cols + first : nullptr;
     const float w = a.w ? a.w[r] : a.mean;
     if (w == 0.f) {
         if (FWD && tid == 0) {
@@ -1072,7 +1076,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 && VPT == 8 && !ACC
 #pragma unroll
         for (int i = 0; i < kEntries; i++)
             if (tid + i * NT < kMaxK) {
-                col_of[tid + i * NT] = col[i];
+                col_of[tid + i * NT] = col[i] - first;  // (columns before the segment come out beyond its end)
                 q_of[tid + i * NT] = f[i] * res.inv_S;
             }
         const float fac = res.empty ? 0.f : res.f, inv_s = res.inv_s;
@@ -1112,122 +1116,59 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 && VPT == 8 && !ACC
     }
 }
 
-// Rows of any length: a workgroup reads the row once for its statistics (a running maximum, the sum rescaled when it grows) and once
-// more for its gradient.
+// The loss of rows of any length: a workgroup reads the row with a running maximum per thread, whose sum is rescaled when it grows.
 constexpr int kStreamNT = 1024;
-template <bool FWD, bool BWD, bool ACC>
-__global__ __launch_bounds__(kStreamNT) void distill_stream_kernel(DistillArgs a) {
-    constexpr int NT = kStreamNT, UP = 2;
-    constexpr uint32_t kSpan = 4 * NT * UP;
-    constexpr int kBits = 13;
-    __shared__ __attribute__((aligned(16))) float span[BWD ? kSpan : 4];
-    __shared__ uint32_t col_of[BWD ? kMaxK : 1];
-    __shared__ float q_of[BWD ? kMaxK : 1];
+__global__ __launch_bounds__(kStreamNT, 8) void distill_stream_kernel(DistillArgs a) {
+    constexpr int NT = kStreamNT, U = 4;
     __shared__ float smem[3 * (NT / kWave)];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+    const int tid = threadIdx.x;
     const uint32_t cols = a.cols, whole = cols & ~3u;
     for (size_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const float* x = a.x + r * cols;
-        float* grad = BWD ? a.grad + r * cols : nullptr;
         const float w = a.w ? a.w[r] : a.mean;
-        __syncthreads();
         if (w == 0.f) {
-            if (FWD && tid == 0) {
-                a.stats[2 * r] = a.stats[2 * r + 1] = 0.f;
-                a.row_loss[r] = 0.f;
-            }
-            if (BWD && !ACC)
-                for (uint32_t c = tid; c < cols; c += NT) grad[c] = 0.f;
+            if (tid == 0) a.stats[2 * r] = a.stats[2 * r + 1] = a.row_loss[r] = 0.f;
             continue;
         }
         uint32_t col;
         float t;
         teacher_entry(a, r, tid, col, t);
-        const float xe = FWD && col != kNoCol ? x[col] : 0.f;
+        const float xe = col != kNoCol ? x[col] : 0.f;
         const float tail = whole + tid < cols ? x[whole + tid] : -INFINITY;
-        float m = -INFINITY, s = 0.f, ls = 0.f;
-        float top[2] = {t, tail};
-        if (FWD) {
-            float mine = -INFINITY;  // this thread's maximum, and its sum from there
-            for (uint32_t c0 = 0; c0 < whole; c0 += 2 * kSpan) {
-                float4u v[2 * UP];
+        float mine = -INFINITY, s = 0.f;  // this thread's maximum, and its sum from there
+        for (uint32_t c0 = 0; c0 < whole; c0 += 4 * NT * U) {
+            float4u v[U];
 #pragma unroll
-                for (int u = 0; u < 2 * UP; u++) v[u] = row_piece(x + c0, bytes_from(c0, whole), 16 * (tid + u * NT));
-                float mx = v[0][0];
+            for (int u = 0; u < U; u++) v[u] = row_piece(x + c0, bytes_from(c0, whole), 16 * (tid + u * NT));
+            float mx = v[0][0];
 #pragma unroll
-                for (int u = 0; u < 2 * UP; u++)
+            for (int u = 0; u < U; u++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mx = fmaxf(mx, v[u][e]);
-                if (mx > mine) {
-                    s = mine == -INFINITY ? s : s * exp2_fast((mine - mx) * a.scale);
-                    mine = mx;
-                }
-                const float from = mine == -INFINITY ? 0.f : mine;
-#pragma unroll
-                for (int u = 0; u < 2 * UP; u++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s += exp2_fast((v[u][e] - from) * a.scale);
+                for (int e = 0; e < 4; e++) mx = fmaxf(mx, v[u][e]);
+            if (mx > mine) {
+                s = mine == -INFINITY ? s : s * exp2_fast((mine - mx) * a.scale);
+                mine = mx;
             }
-            top[1] = fmaxf(top[1], mine);
-            row_maxima<NT, 2>(top, smem);
-            m = top[1];
-            if (mine != -INFINITY) s *= exp2_fast((mine - m) * a.scale);
-        } else {
-            float one[1] = {top[0]};
-            row_maxima<NT, 1>(one, smem);
-            top[0] = one[0];
-            m = a.stats[2 * r];
-            ls = a.stats[2 * r + 1];
+            const float from = mine == -INFINITY ? 0.f : mine;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s += exp2_fast((v[u][e] - from) * a.scale);
         }
+        float top[2] = {t, fmaxf(tail, mine)};
+        row_maxima<NT, 2>(top, smem);
+        const float m = top[1];
+        if (mine != -INFINITY) s *= exp2_fast((mine - m) * a.scale);
         const float from_x = m == -INFINITY ? 0.f : m, from_t = top[0] == -INFINITY ? 0.f : top[0];
-        const float tail_e = exp2_fast((tail - from_x) * a.scale);
         float f, part;
         teacher_terms(a, t, xe, from_t, from_x, f, part);
-        float sum[3] = {f, part, s + tail_e};
+        float sum[3] = {f, part, s + exp2_fast((tail - from_x) * a.scale)};
         row_sums<NT, 3>(sum, smem);
-        const RowResult res = row_result<FWD>(a, w, m, ls, sum[2], sum[0], sum[1]);
-        if (FWD && tid == 0) {
+        const RowResult res = row_result<true>(a, w, m, 0.f, sum[2], sum[0], sum[1]);
+        if (tid == 0) {
             a.stats[2 * r] = res.m;
             a.stats[2 * r + 1] = res.ls;
             a.row_loss[r] = res.loss;
-        }
-        if constexpr (BWD) {
-            if (ACC && res.empty) continue;
-            if (tid < kMaxK) {
-                col_of[tid] = col;
-                q_of[tid] = f * res.inv_S;
-            }
-#pragma unroll
-            for (int u = 0; u < UP; u++) *reinterpret_cast<float4*>(span + 4 * (tid + u * NT)) = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint32_t c0 = 0; c0 < cols; c0 += kSpan) {
-                float4u v[UP], old[UP];
-#pragma unroll
-                for (int u = 0; u < UP; u++) v[u] = row_piece(x + c0, bytes_from(c0, whole), 16 * (tid + u * NT));
-                if (ACC) {
-#pragma unroll
-                    for (int u = 0; u < UP; u++) old[u] = row_piece(grad + c0, bytes_from(c0, whole), 16 * (tid + u * NT));
-                }
-                __syncthreads();
-                if (wave == 0) span_shares(span, col_of, q_of, a.k, c0, kSpan, kBits, tid);
-                __syncthreads();
-                if (whole >= c0 && whole - c0 < kSpan && whole + tid < cols) {
-                    const float d = res.empty ? 0.f : res.f * (tail_e * res.inv_s - span[whole - c0 + tid]);
-                    grad[whole + tid] = ACC ? grad[whole + tid] + d : d;
-                }
-#pragma unroll
-                for (int u = 0; u < UP; u++) {
-                    const uint32_t c = 4 * (tid + u * NT);
-                    if (c0 + c >= whole) continue;
-                    const float4u q = take_shares(span + c);
-                    float4u g;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float d = res.empty ? 0.f : res.f * (exp2_fast((v[u][e] - from_x) * a.scale) * res.inv_s - q[e]);
-                        g[e] = ACC ? old[u][e] + d : d;
-                    }
-                    __builtin_nontemporal_store(g, reinterpret_cast<float4u*>(grad + c0 + c));
-                }
-            }
         }
     }
 }
@@ -1256,15 +1197,34 @@ static int distill_launch(zg_hip_ctx* ctx, const DistillArgs& a, float* loss, bo
         return ZG_HIP_OK;
     }
 #define ZG_ROWS(NT, VPT, UP)                                                                                                          \
-    hipLaunchKernelGGL((distill_row_kernel<NT, VPT, UP, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(a.rows, NT < 256 ? 256 / NT : 1)), \
+    hipLaunchKernelGGL((distill_row_kernel<NT, VPT, UP, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(a.rows * segments, NT < 256 ? 256 / NT : 1)), \
                        dim3(NT < 256 ? 256 : NT), 0, ctx->stream, a)
-    const bool fits = a.rows < 0x7fffffffull && (BWD || a.cols <= 32768);
-    if (fits && a.cols <= 1024) ZG_ROWS(64, 4, 4);
-    else if (fits && a.cols <= 2048) ZG_ROWS(64, 8, 8);
-    else if (fits && a.cols <= 8192) ZG_ROWS(256, 8, 4);
-    else if (fits && a.cols <= 32768) ZG_ROWS(1024, 8, 2);
-    else if (fits && a.cols <= 65536) ZG_ROWS(1024, 16, 2);
-    else hipLaunchKernelGGL((distill_stream_kernel<FWD, BWD, ACC>), dim3(row_grid(a.rows)), dim3(kStreamNT), 0, ctx->stream, a);
+    // a gradient that finds its statistics takes long rows segment by segment
+    const size_t segments = FWD || a.cols <= 2048 ? 1 : ceil_div_sz(a.cols, 8192);
+    ZG_REQUIRE(a.rows * segments < 0x7fffffffull, "distill: %zu rows of %u columns", a.rows, a.cols);
+    if (a.cols <= 1024) {
+        ZG_ROWS(64, 4, 4);
+    } else if (a.cols <= 2048) {
+        ZG_ROWS(64, 8, 8);
+    } else if (!FWD || a.cols <= 8192) {
+        ZG_ROWS(256, 8, 4);
+    } else if constexpr (FWD && BWD) {
+        if (a.cols <= 32768) {
+            ZG_ROWS(1024, 8, 2);
+        } else if (a.cols <= 65536) {
+            ZG_ROWS(1024, 16, 2);
+        } else {
+            // Rows that no workgroup holds: the loss, then the gradient.  (2048 x 128000: 560 us, one kernel that read each row twice
+            // 526; 16 x 128000: 23 us against 36.  Some rows at a time, for the second pass to find them in the memory-side cache,
+            // costs more in half-empty launches than it saves: 619 us.)
+            bool unused;
+            if (int rc = distill_launch<true, false, false>(ctx, a, loss, &unused)) return rc;
+            return distill_launch<false, true, ACC>(ctx, a, loss, &unused);
+        }
+    } else if constexpr (FWD) {
+        if (a.cols <= 32768) ZG_ROWS(1024, 8, 2);
+        else hipLaunchKernelGGL(distill_stream_kernel, dim3(row_grid(a.rows)), dim3(kStreamNT), 0, ctx->stream, a);
+    }
 #undef ZG_ROWS
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
@@ -1345,7 +1305,7 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
 #define ZG_TOPK_SHORT(L, KPL)                                                                                                    \
     hipLaunchKernelGGL((topk_short_kernel<L, KPL>), dim3((unsigned)ceil_div_sz(rows, 256 / (L))), dim3(256), 0, ctx->stream, x,      \
                        values, indices, rows, c32, k32)
-    if (cols <= 256 && k <= 16 && rows < ((size_t)1 << 34)) {
+    if (cols <= 256 && k <= 16) {
         if (cols <= 16) ZG_TOPK_SHORT(4, 4);
         else if (cols <= 64) ZG_TOPK_SHORT(16, 4);
         else if (cols <= 128) ZG_TOPK_SHORT(16, 8);
@@ -1390,7 +1350,7 @@ ZG_API int zg_hip_topk_bwd(zg_hip_ctx* ctx, const uint64_t* indices, const float
         const size_t per_wave = k < kWave ? kWave / k : 1;
         hipLaunchKernelGGL(topk_bwd_add_kernel, dim3(row_grid(ceil_div_sz(rows, 4 * per_wave))), dim3(256), 0, ctx->stream, indices, y_g,
                            x_g, rows, c32, k32, bits);
-    } else if (cols <= 256 && k <= 16 && rows < ((size_t)1 << 34)) {
+    } else if (cols <= 256 && k <= 16) {
         const dim3 grid((unsigned)ceil_div_sz(rows, 16));
         if (cols <= 64) hipLaunchKernelGGL(topk_bwd_short_kernel<1>, grid, dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32);
         else if (cols <= 128) hipLaunchKernelGGL(topk_bwd_short_kernel<2>, grid, dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32);
