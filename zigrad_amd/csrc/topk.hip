@@ -30,7 +30,7 @@ constexpr int kMaxK = ZG_HIP_TOPK_MAX_K;
 //   * values that reach the bound become candidates in LDS as 64-bit keys (value, then column), about k of them among the
 //     first values and k / (4 NT VPT) of the rest of the row.  Each wave has a stretch of LDS and a counter in registers
 //     for its own, so that a candidate costs a ballot and a store (a shared LDS counter, whose answer every store had to
-//     wait for, took 332 us for 64 of 32000 in 8192 rows where this takes 202 us, 5.2 TB/s);
+//     wait for, took 332 us for 64 of 32000 in 8192 rows where this takes 182 us, 5.8 TB/s);
 //   * with more than kRankMost candidates the k largest are cut out by a radix selection over their keys (eight bits at a
 //     time, as many digits as it takes to tell them apart), which also raises the bound for the rest of the row;
 //   * a candidate's place in the result is the number of larger keys, which every thread counts for its own candidates.
@@ -298,12 +298,11 @@ __device__ __forceinline__ void load_tile(float4u (&v)[VPT], const Place& at, co
         v[u] = BEYOND ? __builtin_nontemporal_load(reinterpret_cast<const float4u*>(row) + at.tid + u * NT)
                       : row_piece(row, bytes_from(0, cols & ~3u), 16 * (at.tid + u * NT));
 }
-template <int NT, int VPT, bool BEYOND>
+template <int NT, int VPT, int U, bool BEYOND>
 __device__ __forceinline__ void select_row(Select<NT>& s, Place& at, float4u (&v)[VPT], const float* row, const float* next,
                                            uint32_t cols, uint32_t k) {
     constexpr uint32_t kTile = 4 * NT * VPT;
-    constexpr int U = 4;                    // pieces in flight per thread behind the tile, twice
-    constexpr uint32_t kStep = 4 * NT * U;  // their columns
+    constexpr uint32_t kStep = 4 * NT * U;  // columns of the pieces that are looked through or on their way at a time
     const uint32_t whole = cols & ~3u;
     // behind the tile a step of pieces is looked through while the next one is on its way
     float4u w[2][U];
@@ -440,8 +439,8 @@ __device__ __forceinline__ void select_emit(Select<NT>& s, Place& at, uint32_t k
     }
 }
 
-template <int NT, int VPT, bool BEYOND>
-__global__ __launch_bounds__(256, 4) void topk_kernel(const float* x, float* values, uint64_t* indices, size_t rows, uint32_t cols,
+template <int NT, int VPT, int U, bool BEYOND>
+__global__ __launch_bounds__(256, U > 4 ? 3 : 4) void topk_kernel(const float* x, float* values, uint64_t* indices, size_t rows, uint32_t cols,
                                                       uint32_t k) {
     constexpr int kRows = 256 / NT;
     __shared__ Select<NT> mem[kRows];
@@ -456,7 +455,7 @@ __global__ __launch_bounds__(256, 4) void topk_kernel(const float* x, float* val
     load_tile<NT, VPT, BEYOND>(v, at, x + r * cols, cols);
     for (; r < rows; r += step) {
         const float* row = x + r * cols;
-        select_row<NT, VPT, BEYOND>(s, at, v, row, r + step < rows ? x + (r + step) * cols : nullptr, cols, k);
+        select_row<NT, VPT, U, BEYOND>(s, at, v, row, r + step < rows ? x + (r + step) * cols : nullptr, cols, k);
         select_emit<NT>(s, at, k, [&](uint32_t rank, uint64_t key) {
             const uint32_t c = ~(uint32_t)key;
             float v = key_value((uint32_t)(key >> 32));
@@ -479,7 +478,7 @@ __global__ __launch_bounds__(256, 4) void topk_segments_kernel(const float* x, u
     const float* part = x + r * cols + c0;
     float4u v[4];
     load_tile<256, 4, false>(v, at, part, n);
-    select_row<256, 4, false>(s, at, v, part, nullptr, n, k);
+    select_row<256, 4, 4, false>(s, at, v, part, nullptr, n, k);
     select_emit<256>(s, at, k, [&](uint32_t rank, uint64_t key) {
         keys[((size_t)blockIdx.x) * k + rank] = (key & ~(uint64_t)0xffffffffu) | (uint32_t)~(~(uint32_t)key + c0);
     });
@@ -1274,12 +1273,12 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
                "topk_fwd: an output overlaps another operand");
     DeviceGuard guard(ctx);
     const uint32_t c32 = (uint32_t)cols, k32 = (uint32_t)k;
-#define ZG_TOPK(NT, VPT, BEYOND)                                                                                      \
-    hipLaunchKernelGGL((topk_kernel<NT, VPT, BEYOND>), dim3(grid(256 / (NT))), dim3(256), 0, ctx->stream, x, values,       \
+#define ZG_TOPK(NT, VPT, U, BEYOND)                                                                                      \
+    hipLaunchKernelGGL((topk_kernel<NT, VPT, U, BEYOND>), dim3(grid(256 / (NT), U)), dim3(256), 0, ctx->stream, x, values,       \
                        indices, rows, c32, k32)
     // as many workgroups as the compute units hold, with the same number of rows each
-    auto grid = [&](size_t per_block) {
-        const size_t blocks = ceil_div_sz(rows, per_block), most = (size_t)ctx->n_cu * 4;
+    auto grid = [&](size_t per_block, int u) {
+        const size_t blocks = ceil_div_sz(rows, per_block), most = (size_t)ctx->n_cu * (u > 4 ? 3 : 4);
         return (unsigned)ceil_div_sz(blocks, ceil_div_sz(blocks, most));
     };
     // A few long rows are cut into segments, which takes two launches (64 of 128000: 1 row 16 us against 39 us with a workgroup per
@@ -1311,19 +1310,20 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
         else if (cols <= 128) ZG_TOPK_SHORT(16, 8);
         else ZG_TOPK_SHORT(16, 16);
     } else if (k <= 128 && (cols <= 2048 || rows >= (size_t)ctx->n_cu * 8)) {
-        if (cols <= 256) ZG_TOPK(64, 1, false);
-        else if (cols <= 512) ZG_TOPK(64, 2, false);
-        else if (cols <= 1024) ZG_TOPK(64, 4, false);
-        else if (cols <= 2048) ZG_TOPK(64, 8, false);
-        else ZG_TOPK(64, 8, true);
+        if (cols <= 256) ZG_TOPK(64, 1, 4, false);
+        else if (cols <= 512) ZG_TOPK(64, 2, 4, false);
+        else if (cols <= 1024) ZG_TOPK(64, 4, 4, false);
+        else if (cols <= 2048) ZG_TOPK(64, 8, 4, false);
+        else if (cols <= 8192) ZG_TOPK(64, 8, 4, true);
+        else ZG_TOPK(64, 4, 6, true);  // fewer waves with more on its way each (64 of 32000 in 8192 rows: 182 us against 202)
     } else if (cols <= 2048) {
-        ZG_TOPK(256, 2, false);
+        ZG_TOPK(256, 2, 4, false);
     } else if (cols <= 4096) {
-        ZG_TOPK(256, 4, false);
+        ZG_TOPK(256, 4, 4, false);
     } else if (cols <= 8192) {
-        ZG_TOPK(256, 8, false);
+        ZG_TOPK(256, 8, 4, false);
     } else {
-        ZG_TOPK(256, 8, true);
+        ZG_TOPK(256, 8, 4, true);
     }
 #undef ZG_TOPK_SHORT
 #undef ZG_TOPK
