@@ -48,9 +48,9 @@ int zg_hip_topk_bwd(zg_hip_ctx *ctx, const uint64_t *indices, const float *y_g, 
  * 0, whatever its logits hold) when its weight is 0, when it has no teacher logit above -inf, or when all its logits
  * are -inf.  A class of p = 0 that the teacher wants (q > 0) makes the row's loss infinite and leaves its gradient finite.
  * stats[r, :] = { max_c logits, log sum_c exp((logits - max) / temperature) }, {-inf, 0} for a row whose logits are all -inf,
- * {0, 0} for a row of weight 0 (its logits are not read): what zg_hip_distill_bwd needs of the row.  temperature > 0 and finite; cols < 2^31.  As with the other
- * losses the forward calls refuse an empty matrix and the backward does nothing on one.  Rows longer than a workgroup's
- * share of a small batch use the workspace.
+ * {0, 0} for a row of weight 0 (its logits are not read): what zg_hip_distill_bwd needs of the row.  1e-18 <=
+ * temperature <= 1e18; cols < 2^31.  As with the other losses the forward calls refuse an empty matrix and the backward does
+ * nothing on one.
  * ------------------------------------------------------------------------------------------- */
 int zg_hip_distill_fwd(zg_hip_ctx *ctx, const float *logits, const float *teacher, const uint64_t *indices,
                        const float *row_weights, float *stats, float *row_loss, float *loss, size_t rows, size_t cols,
@@ -99,7 +99,7 @@ int zg_hip_expert_combine_bwd(zg_hip_ctx *ctx, const float *out_g, const float *
  *   forward   y = x w_e^T + bias_e (null: none), max(0, .) when relu
  *   backward  gw_e += gy_e^T x_e;  gb_e += column sums of gy_e (null: none);  gx = gy w_e, zero where act_in <= 0 (gx null: no
  *             input gradient, w is not read; act_in null: no mask).  accumulate == 0: gw and gb are written, zero for an
- *             expert without rows.
+ *             expert without rows.  A layer without inputs or outputs: nothing to do.  Uses the workspace when there are more than 64 experts or gb is given.
  * ------------------------------------------------------------------------------------------- */
 int zg_hip_expert_linear_fwd(zg_hip_ctx *ctx, const float *x, const float *w, const float *bias, float *y,
                              const uint64_t *offsets, size_t n_rows, size_t n_experts, size_t fan_in, size_t fan_out, int relu);

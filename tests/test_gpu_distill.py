@@ -84,6 +84,36 @@ def test_many_rows(hip, rows, cols, k, fused):
     check(run(hip, x, teacher, indices, 2.0, None, grad0, fused), x, teacher, indices, 2.0, None, grad0)
 
 
+@pytest.mark.parametrize("cols", [8192, 8196, 16385, 32764, 32768, 65532, 65536, 65537, 65541])
+@pytest.mark.parametrize("fused", [False, True])
+def test_row_lengths_around_the_kernels_own(hip, cols, fused):
+    x, teacher, indices, grad0 = case(cols, 3, cols, 20)
+    w = np.array([0.25, 0.0, 0.5], np.float32)
+    for add in (None, grad0):
+        check(run(hip, x, teacher, indices, 2.0, w, add, fused), x, teacher, indices, 2.0, w, add)
+
+
+@pytest.mark.parametrize("cols", [10, 200, 5000, 33000, 70000])
+def test_extreme_temperatures(hip, cols):
+    """At 1e-18 every row but those of equal logits has one class; at 1e18 all classes are equal and the loss is next to nothing."""
+    x, teacher, indices, _ = case(cols, 3, cols, 4)
+    x[:, :4], teacher[:], indices[:] = 0, 0, np.arange(4)
+    x[:, 4:] = -1 - np.abs(x[:, 4:])
+    for fused in (False, True):
+        got = run(hip, x, teacher, indices, 1e-18, None, None, fused)
+        assert (got["stats"][:, 0] == 0).all() and np.abs(got["stats"][:, 1] - np.log(4)).max() <= 4 * EPS * np.log(4)
+        assert np.abs(got["row_loss"]).max() <= 1e-36 and np.abs(got["grad"][:, :4]).max() <= 1e-18
+        assert (got["grad"][:, 4:] == 0).all()
+        got = run(hip, x, teacher, indices, 1e18, None, None, fused)
+        # gradient: temperature / rows (1 / cols - [kept] / 4).  p = exp(-log cols): the logarithm, its difference and the argument
+        # of the exponential are off by 5 halves of a step of log cols together, the exponential and the factors by 8 of p;
+        # q and its factors by 16 of q
+        p, q = np.full((3, cols), 1 / cols), np.zeros((3, cols))
+        q[:, :4] = 0.25
+        slack = (p * (5 * np.log(cols) + 8) + 16 * q + 2 * np.abs(p - q)) * EPS
+        assert (np.abs(got["grad"] / (1e18 / 3) - (p - q)) <= slack).all()
+
+
 @pytest.mark.parametrize("temp", [0.05, 0.5, 1.0, 3.0, 20.0])
 @pytest.mark.parametrize("cols", [12, 700, 9000])
 def test_temperatures(hip, temp, cols):

@@ -189,6 +189,56 @@ def test_a_recorded_step_replays_what_eager_calls_leave(hip):
     s.free()
 
 
+@pytest.mark.parametrize("op", ["topk_fwd", "expert_sort", "expert_linear_bwd"])
+def test_a_recording_without_a_run_before_it(hip, op):
+    """A call that would have to allocate its workspace is refused in a recording; the context and the recording go on."""
+    dev = HipDevice(0)  # no workspace yet
+    try:
+        if op == "topk_fwd":
+            x = np.random.default_rng(1).standard_normal((2, 40000)).astype(F32)
+            b = dict(x=dev.from_numpy(x), values=dev.mem_alloc(F32, 16), indices=dev.mem_alloc(U64, 16))
+            size = dict(rows=2, cols=40000, k=8)
+        elif op == "expert_sort":
+            experts = np.random.default_rng(1).integers(0, 9, 5000).astype(U64)
+            b = dict(experts=dev.from_numpy(experts), offsets=dev.mem_alloc(U64, 10), slots=dev.mem_alloc(U64, 5000))
+            size = dict(n_experts=9)
+        else:
+            b = dict(offsets=dev.from_numpy((np.arange(71) * 12).astype(U64)), gb=dev.mem_alloc(F32, 70 * 8), w=None, act_in=None, gx=None,
+                     **{n: dev.from_numpy(np.ones(840 * 8, F32)) for n in ("gy", "x")}, gw=dev.mem_alloc(F32, 70 * 64))
+            size = dict(n_rows=840, n_experts=70, fan_in=8, fan_out=8, accumulate=False)
+        other = dev.from_numpy(np.ones(4, F32))
+        dev.sync()
+        dev.graph_open()
+        try:
+            with pytest.raises(RuntimeError):
+                dev.dispatch(op, **b, **size)
+            dev.dispatch("scale", x=other, alpha=2.0)
+        finally:
+            graph = dev.graph_save()
+        graph.run()
+        graph.run()
+        assert (dev.to_numpy(other) == 4).all()
+        dev.dispatch(op, **b, **size)  # eagerly: the workspace is there now
+        graph.free()
+        dev.sync()
+        dev.graph_open()
+        try:
+            dev.dispatch(op, **b, **size)
+        finally:
+            graph = dev.graph_save()
+        out = {"topk_fwd": "indices", "expert_sort": "slots", "expert_linear_bwd": "gw"}[op]
+        want = dev.to_numpy(b[out])
+        for _ in range(2):
+            dev.mem_fill(b[out], 77)
+            graph.run()
+            assert np.array_equal(dev.to_numpy(b[out]), want)
+        if op == "expert_linear_bwd":
+            assert (want == 12).all()
+        graph.free()
+    finally:
+        dev.deinit()
+
+
 def test_two_contexts_at_once(hip):
     """Each context orders and multiplies on its own stream with its own workspace."""
     steps = [Step(tokens=3000, width=40, hidden=56, classes=65, experts=32, k=4, kept=8, seed=7), None]

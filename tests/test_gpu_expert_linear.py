@@ -136,6 +136,57 @@ def test_ordinary_layers(hip, n, e, fan_in, fan_out):
     check_bwd(hip, c, True, True, False)
 
 
+@pytest.mark.parametrize("n_experts,per,fan_in,fan_out", [(65, 12, 50, 70), (1024, 10, 17, 33), (24, 12, 1020, 1024), (67, 9, 637, 640)])
+def test_many_experts_of_many_rows(hip, n_experts, per, fan_in, fan_out):
+    """The experts' order found by a launch of its own (more than 64), the large tiles of the weight gradients."""
+    r = np.random.default_rng(n_experts)
+    counts = r.integers(0, 2 * per, n_experts)
+    counts[::5] = 0
+    counts[1] += 3 * per
+    counts[0] = max(0, n_experts * per - int(counts.sum()))
+    c = case(n_experts, counts, 1, fan_in, fan_out)
+    assert c["n"] // n_experts > 8
+    check_fwd(hip, c, True, True)
+    check_bwd(hip, c, True, True, True)
+    check_bwd(hip, c, False, False, False, shift=1)
+
+
+@pytest.mark.parametrize("per", [2, 3, 6, 7, 16, 17, 20, 21, 32, 33, 48, 49])
+@pytest.mark.parametrize("n_experts,fan_in,fan_out", [(8, 64, 96), (16, 520, 260), (40, 96, 516)])
+def test_rows_per_expert(hip, n_experts, fan_in, fan_out, per):
+    """The average number of rows decides between the kernels for few rows and the tiled ones; some experts have other numbers."""
+    r = np.random.default_rng(per)
+    counts = np.full(n_experts, per)
+    counts[1], counts[3] = 0, 2 * per
+    counts[5:8] = r.multinomial(3 * per, [0.7, 0.2, 0.1])
+    c = case(per, counts, 0, fan_in, fan_out)
+    check_fwd(hip, c, True, True)
+    check_bwd(hip, c, True, True, True, shift=per % 2)
+
+
+@pytest.mark.parametrize("counts,fan_in,fan_out", [([3, 5, 2, 4], 40, 36), ([30, 21, 50, 18], 70, 66), ([300, 120, 500, 200], 132, 200)])
+def test_one_expert_of_nan_leaves_the_others_alone(hip, counts, fan_in, fan_out):
+    c = case(5, counts, 0, fan_in, fan_out)
+    offsets = c["offsets"].astype(int)
+    bad = slice(offsets[2], offsets[3])
+    out = {}
+    for kind in ("clean", "nan"):
+        if kind == "nan":
+            c["x"][bad], c["gy"][bad], c["w"][2], c["b"][2] = np.nan, np.inf, -np.inf, np.nan
+        b = {n: hip.from_numpy(c[n]) for n in ("x", "w", "b", "gy", "act", "offsets")}
+        y, gw, gb, gx = (hip.from_numpy(np.zeros(s, np.float32)) for s in (c["gy"].shape, c["w"].shape, c["b"].shape, c["x"].shape))
+        layer = dict(offsets=b["offsets"], n_rows=c["n"], n_experts=4, fan_in=fan_in, fan_out=fan_out)
+        hip.dispatch("expert_linear_fwd", x=b["x"], w=b["w"], bias=b["b"], y=y, relu=False, **layer)
+        hip.dispatch("expert_linear_bwd", gy=b["gy"], x=b["x"], w=b["w"], act_in=b["act"], gw=gw, gb=gb, gx=gx, accumulate=False, **layer)
+        out[kind] = [hip.to_numpy(y, c["gy"].shape), hip.to_numpy(gw, c["w"].shape), hip.to_numpy(gb, c["b"].shape), hip.to_numpy(gx, c["x"].shape)]
+    others = np.ones(c["n"], bool)
+    others[bad] = False
+    for i, (clean, nan) in enumerate(zip(out["clean"], out["nan"])):
+        keep = others if i in (0, 3) else np.array([True, True, False, True])
+        assert np.array_equal(clean[keep], nan[keep]), i
+        assert not np.isfinite(nan[~keep]).all(), i
+
+
 def test_offsets_that_make_no_sense_stay_inside_the_rows(hip):
     """Ranges beyond n_rows end there, ranges that end before they begin are empty."""
     c = case(3, [10, 20, 30], 0, 20, 24)

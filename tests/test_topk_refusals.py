@@ -46,7 +46,8 @@ BAD = {
                            (dict(row_loss=0), "null"), (dict(loss=0), "null"), (dict(indices=C + 4), "8-byte"),
                            (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"),
                            (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature"),
-                           (dict(temperature=1e-45), "temperature"), (dict(stats=A), "overlaps"), (dict(row_loss=D), "overlaps"),
+                           (dict(temperature=1e-45), "temperature"), (dict(temperature=9e-19), "temperature"),
+                           (dict(temperature=1.1e18), "temperature"), (dict(stats=A), "overlaps"), (dict(row_loss=D), "overlaps"),
                            (dict(loss=F + 12), "overlap"), (dict(row_loss=E + 16), "overlap"), (dict(cols=1 << 33), "columns"),
                            (dict(rows=1 << 58), "rows")],
     "zg_hip_distill_bwd": [(dict(k=0), "k = 0"), (dict(stats=0), "null"), (dict(grad=0), "null"), (dict(grad=A), "overlaps"),

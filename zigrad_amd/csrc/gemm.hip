@@ -2793,9 +2793,9 @@ __global__ __launch_bounds__(256, 4) void expert_weights_few_kernel(const float*
     expert_range(offsets, blockIdx.z, n_rows, first, count);
     first = (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
     count = (uint32_t)__builtin_amdgcn_readfirstlane((int)count);
-    const size_t c = ((size_t)blockIdx.x * tx + threadIdx.x % tx) * 4;
+    const size_t c = ((size_t)blockIdx.y * tx + threadIdx.x % tx) * 4;
     // a wave's threads share their outputs (tx is a multiple of 64), so what they read of gy is the same for all
-    const size_t o0 = ((size_t)blockIdx.y * (256 / tx) + (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / tx))) * kFewOuts;
+    const size_t o0 = ((size_t)blockIdx.x * (256 / tx) + (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / tx))) * kFewOuts;
     if (c >= fan_in || o0 >= fan_out) return;
     const int outs = fan_out - o0 < kFewOuts ? (int)(fan_out - o0) : kFewOuts;
     const bool whole = c + 4 <= fan_in;
@@ -2998,8 +2998,7 @@ ZG_API int zg_hip_expert_linear_bwd(zg_hip_ctx* ctx, const float* gy, const floa
     if (few) {
         int tx = 64;
         while (tx < 256 && (size_t)tx * 4 < fan_in) tx *= 2;
-        const dim3 grid((unsigned)ceil_div_sz(fan_in, 4 * tx), (unsigned)ceil_div_sz(fan_out, 256 / tx * kFewOuts), (unsigned)n_experts);
-        ZG_REQUIRE(grid.y < 65536, "expert_linear_bwd: %zu outputs", fan_out);
+        const dim3 grid((unsigned)ceil_div_sz(fan_out, 256 / tx * kFewOuts), (unsigned)ceil_div_sz(fan_in, 4 * tx), (unsigned)n_experts);
         if (accumulate)
             hipLaunchKernelGGL(expert_weights_few_kernel<true>, grid, dim3(256), 0, ctx->stream, gy, x, gw, offsets, n_rows, fan_in, fan_out, tx);
         else

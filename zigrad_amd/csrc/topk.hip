@@ -1237,7 +1237,8 @@ static int distill_check(const char* op, const float* logits, const float* teach
     ZG_REQUIRE(cols < ((size_t)1 << 31), "%s: %zu columns", op, cols);
     ZG_REQUIRE(mul_sat(rows, cols) < ((size_t)1 << 60) && mul_sat(rows, k) < ((size_t)1 << 60), "%s: %zu rows", op, rows);
     ZG_REQUIRE(k >= 1 && k <= kMaxK, "%s: k = %zu is not in 1 .. %d", op, k, kMaxK);
-    ZG_REQUIRE(temperature > 0.f && temperature < INFINITY && 1.f / temperature < 1e38f, "%s: temperature %g", op, temperature);
+    // its square and its inverse are normal numbers
+    ZG_REQUIRE(temperature >= 1e-18f && temperature <= 1e18f, "%s: temperature %g is not in 1e-18 .. 1e18", op, temperature);
     return ZG_HIP_OK;
 }
 // an output against the inputs of the loss
