@@ -151,6 +151,20 @@ def test_many_experts_of_many_rows(hip, n_experts, per, fan_in, fan_out):
     check_bwd(hip, c, False, False, False, shift=1)
 
 
+@pytest.mark.parametrize("n,e,fan_in,fan_out", [(4500, 70, 68, 1920), (10500, 5, 302, 1660), (2700, 3, 200, 6143)])
+def test_wide_tiles(hip, n, e, fan_in, fan_out):
+    """Enough tiles of 64 x 128 for all compute units, forward or in the input gradient, the last column of tiles whole or not."""
+    r = np.random.default_rng(n)
+    share = r.random(e) ** 2
+    counts = np.floor(share / share.sum() * (n - 7)).astype(int)
+    c = case(n, counts, n - int(counts.sum()), fan_in, fan_out)
+    check_fwd(hip, c, True, True)
+    check_fwd(hip, c, True, False, shift=1)
+    c = case(n + 1, counts, n - int(counts.sum()), fan_out, fan_in)
+    check_bwd(hip, c, True, True, False)
+    check_bwd(hip, c, False, False, True, shift=3)
+
+
 @pytest.mark.parametrize("per", [2, 3, 6, 7, 16, 17, 20, 21, 32, 33, 48, 49])
 @pytest.mark.parametrize("n_experts,fan_in,fan_out", [(8, 64, 96), (16, 520, 260), (40, 96, 516)])
 def test_rows_per_expert(hip, n_experts, fan_in, fan_out, per):

@@ -2763,8 +2763,12 @@ static int expert_rows(zg_hip_ctx* ctx, const float* A, const float* B, float* C
         if (per <= 2 || (per <= 16 && tiles <= n_cu)) return launch_expert_few<1, 1, 8, B_KMAJOR>(ctx, g);
         if (per <= 32 && tiles <= 3 * n_cu) return launch_expert_few<2, 2, 4, B_KMAJOR>(ctx, g);
     }
-    // 64 x 64 tiles: the larger ones waste more on the last tile of every expert than they gain (16384 rows, 16 experts, 1024 -> 2048:
-    // 536 us, 128 x 128 533, 256 x 128 595; 64 experts, 1024 -> 1024: 308, 356 and 473 us)
+    // 64 x 128 tiles where eight a compute unit average out and the last column of tiles is as full as with 64 x 64 (1024 -> 2048, 16
+    // experts: 16384 rows 543 -> 520 us, 8192 rows 282 -> 274, 6000 rows 213 -> 212; 1024 -> 1088: 289 -> 301).  Taller ones waste
+    // more on the last tile of every expert than they gain (16384 rows: 128 x 64 532 us, 128 x 128 533; 65536 rows, 64 experts, 1024
+    // -> 1024: 64 x 64 1112, 64 x 128 1059, 128 x 64 1099, 128 x 128 1075).
+    const size_t wide = (n_rows / 64 + (n_rows < n_experts ? n_rows : n_experts)) * ceil_div_sz(n, 128);
+    if (wide >= 8 * n_cu && ceil_div_sz(n, 64) % 2 == 0) return launch_expert_rows<64, 128, B_KMAJOR>(ctx, g);
     return launch_expert_rows<64, 64, B_KMAJOR>(ctx, g);
 }
 // C_e (+)= A[rows of e]^T B[rows of e]
