@@ -86,9 +86,10 @@ struct Place {
 // there.  Pieces behind that are -inf, which loses to every value of the row: a buffer load takes any 4-byte alignment and
 // reads nothing behind the end.
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+template <bool ONCE = false>  // ONCE: nothing will read it again soon
 __device__ __forceinline__ float4u row_piece(const float* base, uint32_t bytes, uint32_t off) {
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, (int)bytes, 0x00020000);
-    const float4u v = __builtin_bit_cast(float4u, (uint4v)__builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, 0));
+    const float4u v = __builtin_bit_cast(float4u, (uint4v)__builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, ONCE ? 2 : 0));
     const bool in = off < bytes;
     return float4u{in ? v.x : -INFINITY, in ? v.y : -INFINITY, in ? v.z : -INFINITY, in ? v.w : -INFINITY};
 }
@@ -740,6 +741,7 @@ struct DistillArgs {
     size_t rows;
     uint32_t cols, k;
     float temp, inv_temp, scale, mean;  // scale = log2(e) / temp
+    uint32_t segments, segment;         // the gradient alone: parts of a row, and their columns
 };
 
 // the hardware's 2^x: off by a step at most, which with the roundings of its argument is what exp(x) of a library has lost as well
@@ -941,12 +943,11 @@ __global__ __launch_bounds__(NTB) void distill_short_kernel(DistillArgs a, float
     }
 }
 
-// The q_j of the columns [c0, c0 + n) into the stretch of zeros `span`, by one wave, in the order of j.
-__device__ __forceinline__ void span_shares(float* span, const uint32_t* col, const float* q, uint32_t k, uint32_t c0, uint32_t n, int bits,
-                                            int lane) {
+// The q_j into the stretch of n zeros `span`, by one wave, in the order of j.
+__device__ __forceinline__ void span_shares(float* span, const uint32_t* col, const float* q, uint32_t k, uint32_t n, int bits, int lane) {
     for (uint32_t j0 = 0; j0 < k; j0 += kWave) {
-        const uint32_t at = (j0 + lane < k ? col[j0 + lane] : kNoCol) - c0;
-        const bool here = at < n;  // (kNoCol - c0 is beyond: rows are shorter than 2^31)
+        const uint32_t at = j0 + lane < k ? col[j0 + lane] : kNoCol;
+        const bool here = at < n;
         const uint64_t heres = __ballot(here);
         if (!heres) continue;
         uint64_t same = same_lanes(here ? at : 0u, bits, heres);
@@ -955,20 +956,16 @@ __device__ __forceinline__ void span_shares(float* span, const uint32_t* col, co
         select_sync<kWave>();
     }
 }
-// four values of the gradient; clears what it takes from the stretch
-__device__ __forceinline__ float4u take_shares(float* at) {
-    const float4 s = *reinterpret_cast<const float4*>(at);
-    if (s.x != 0.f || s.y != 0.f || s.z != 0.f || s.w != 0.f) *reinterpret_cast<float4*>(at) = make_float4(0.f, 0.f, 0.f, 0.f);
-    return float4u{s.x, s.y, s.z, s.w};
-}
 
-// NT threads a row (a wave: four rows a workgroup), which they hold in VPT pieces of four columns each; the gradient leaves UP pieces
-// per thread at a time.
-template <int NT, int VPT, int UP, bool FWD, bool BWD, bool ACC>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 && VPT == 8 && !ACC ? 8 : 1) void distill_row_kernel(DistillArgs a) {
+// NT threads a row (a wave: four rows a workgroup), which they hold in VPT pieces of four columns each.  The gradient (of rows of a wave
+// only) takes its shares from a stretch of LDS.
+template <int NT, int VPT, bool FWD, bool BWD, bool ACC>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 ? 8 : 1) void distill_row_kernel(DistillArgs a) {
+    static_assert(!BWD || NT == kWave, "one wave fills the stretch and reads it");
     constexpr int kRows = NT < 256 ? 256 / NT : 1;
-    constexpr uint32_t kSpan = 4 * NT * UP;
-    constexpr int kBits = 2 + (NT == 64 ? 6 : NT == 256 ? 8 : 10) + (UP == 1 ? 0 : UP == 2 ? 1 : UP == 4 ? 2 : 3);
+    constexpr uint32_t kSpan = 4 * NT * VPT;
+    constexpr int kBits = VPT == 4 ? 10 : 11;
+    static_assert(!BWD || kSpan == 1u << kBits, "bits of a column");
     constexpr int kEntries = (kMaxK + NT - 1) / NT;
     __shared__ __attribute__((aligned(16))) float span_mem[BWD ? kRows * kSpan : 4];
     __shared__ uint32_t col_mem[BWD ? kRows * kMaxK : 1];
@@ -979,15 +976,11 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 && VPT == 8 && !ACC
     float* const span = span_mem + (BWD ? sub * kSpan : 0);
     uint32_t* const col_of = col_mem + (BWD ? sub * kMaxK : 0);
     float* const q_of = q_mem + (BWD ? sub * kMaxK : 0);
-    // The gradient alone, whose statistics are known, is done segment by segment of a long row (first, cols: this one's columns).
-    const size_t job = (size_t)blockIdx.x * kRows + sub;
-    const uint32_t segments = FWD ? 1u : (a.cols - 1) / (4 * NT * VPT) + 1;
-    const size_t r = FWD ? job : job / segments;
+    const size_t r = (size_t)blockIdx.x * kRows + sub;
     if (r >= a.rows) return;  // only waves that own a row of their own: no barrier is missed
-    const uint32_t first = FWD ? 0u : (uint32_t)(job - r * segments) * (4 * NT * VPT);
-    const uint32_t cols = FWD || a.cols - first < 4 * NT * VPT ? a.cols - first : 4 * NT * VPT, whole = cols & ~3u;
-    const float* x = a.x + r * a.cols + first;
-    float* grad = BWD ? a.grad + r * a.cols + first : nullptr;
+    const uint32_t cols = a.cols, whole = cols & ~3u;
+    const float* x = a.x + r * cols;
+    float* grad = BWD ? a.grad + r * cols : nullptr;
     const float w = a.w ? a.w[r] : a.mean;
     if (w == 0.f) {
         if (FWD && tid == 0) {
@@ -1021,7 +1014,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 && VPT == 8 && !ACC
     }
     if (BWD) {
 #pragma unroll
-        for (int u = 0; u < UP; u++) *reinterpret_cast<float4*>(span + 4 * (tid + u * NT)) = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int u = 0; u < VPT; u++) *reinterpret_cast<float4*>(span + 4 * (tid + u * NT)) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     float m, ls;
     if (FWD) {
@@ -1073,46 +1066,233 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 && VPT == 8 && !ACC
     if constexpr (BWD) {
         if (ACC && res.empty) return;
 #pragma unroll
-        for (int i = 0; i < kEntries; i++)
-            if (tid + i * NT < kMaxK) {
-                col_of[tid + i * NT] = col[i] - first;  // (columns before the segment come out beyond its end)
-                q_of[tid + i * NT] = f[i] * res.inv_S;
-            }
+        for (int i = 0; i < kEntries; i++) {
+            col_of[tid + i * NT] = col[i];
+            q_of[tid + i * NT] = f[i] * res.inv_S;
+        }
         const float fac = res.empty ? 0.f : res.f, inv_s = res.inv_s;
-        float4u share_t = {0.f, 0.f, 0.f, 0.f};
+        float4u old[VPT];
+        if (ACC) {
 #pragma unroll
-        for (int ph = 0; ph < VPT / UP; ph++) {
-            const uint32_t c0 = ph * kSpan;
-            if (c0 >= cols) break;
-            select_sync<NT>();
-            if (NT == kWave || wave == 0)
-                span_shares(span, col_of, q_of, a.k, c0, kSpan, kBits, threadIdx.x % kWave);
-            float4u old[UP];
-            if (ACC) {
+            for (int u = 0; u < VPT; u++) old[u] = row_piece(grad, bytes_from(0, whole), 16 * (tid + u * NT));
+        }
+        select_sync<NT>();
+        span_shares(span, col_of, q_of, a.k, kSpan, kBits, tid);
+        select_sync<NT>();
 #pragma unroll
-                for (int u = 0; u < UP; u++) old[u] = row_piece(grad + c0, bytes_from(c0, whole), 16 * (tid + u * NT));
+        for (int u = 0; u < VPT; u++) {
+            const uint32_t c = 4 * (tid + u * NT);
+            if (c >= whole) continue;
+            const float4 q = *reinterpret_cast<const float4*>(span + c);
+            const float4u share = {q.x, q.y, q.z, q.w};
+            float4u g;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float d = res.empty ? 0.f : fac * (v[u][e] * inv_s - share[e]);
+                g[e] = ACC ? old[u][e] + d : d;
             }
-            select_sync<NT>();
-            if (whole >= c0 && whole - c0 < kSpan && whole + tid < cols) share_t[0] = span[whole - c0 + tid];
-#pragma unroll
-            for (int u = 0; u < UP; u++) {
-                const uint32_t c = 4 * (tid + u * NT);
-                if (c0 + c >= whole) continue;  // the tail's shares are for the first threads
-                const float4u q = take_shares(span + c);
-                float4u g;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float d = res.empty ? 0.f : fac * (v[ph * UP + u][e] * inv_s - q[e]);
-                    g[e] = ACC ? old[u][e] + d : d;
-                }
-                __builtin_nontemporal_store(g, reinterpret_cast<float4u*>(grad + c0 + c));
-            }
+            __builtin_nontemporal_store(g, reinterpret_cast<float4u*>(grad + c));
         }
         if (whole + tid < cols) {
-            const float d = res.empty ? 0.f : fac * (tail_e * inv_s - share_t[0]);
+            const float d = res.empty ? 0.f : fac * (tail_e * inv_s - span[whole + tid]);
             grad[whole + tid] = ACC ? grad[whole + tid] + d : d;
         }
     }
+}
+
+// The gradient of rows of more than 2048 columns, with the loss (FWD) by a workgroup for the whole row, without it (the statistics are
+// known) by one for each segment of a row.  R pieces of four columns a thread are held in registers and L in LDS.  A stretch of
+// shares would cost a barrier for every part of the row it covers: the gradient is written without them, and once that is done the thread
+// of the first of a class's entries writes the class's gradient again, from the logit that it read.
+// Rows of 32769 to 53248 columns fit twice on a compute unit that way, so that one is read or written while the other is summed
+// up.  (2048 x 50257, k = 100: 165 us against 189 with the row in registers and shares from LDS; 8192 x 32000: 355 against 394; added
+// to an old gradient, whose pieces take the registers: 221 against 250 and 496 against 581.)
+template <int NT, int R, int L, bool FWD, bool ACC>
+__global__ __launch_bounds__(NT, R <= (ACC ? 4 : 9) ? 8 : 4) void distill_grad_kernel(DistillArgs a) {
+    static_assert(!ACC || L == 0, "old pieces of those in LDS");
+    constexpr uint32_t kCols = 4 * NT * (R + L);
+    constexpr int kEntries = (kMaxK + NT - 1) / NT;
+    constexpr int kBatch = ACC ? (R < 8 ? R : 8) : 1;  // old pieces on their way at a time, the first before the sums
+    __shared__ float4 held[L ? L * NT : 1];
+    __shared__ uint32_t col_of[kMaxK];
+    __shared__ float q_of[kMaxK];
+    __shared__ float smem[3 * (NT / kWave)];
+    __shared__ uint32_t named[kCols / 32];  // a bit for each class
+    __shared__ uint32_t twice;              // whether one is named twice
+    const int tid = threadIdx.x;
+    const size_t r = FWD ? blockIdx.x : blockIdx.x / a.segments;
+    const uint32_t first = FWD ? 0u : (uint32_t)(blockIdx.x - r * a.segments) * a.segment;
+    const uint32_t cols = FWD || a.cols - first < a.segment ? a.cols - first : a.segment, whole = cols & ~3u;
+    const float* x = a.x + r * a.cols + first;
+    float* grad = a.grad + r * a.cols + first;
+    const float w = a.w ? a.w[r] : a.mean;
+    auto zeros = [&] {
+        for (uint32_t c = 4 * tid; c < whole; c += 4 * NT) *reinterpret_cast<float4u*>(grad + c) = float4u{0.f, 0.f, 0.f, 0.f};
+        if (whole + tid < cols) grad[whole + tid] = 0.f;
+    };
+    if (w == 0.f) {
+        if (FWD && tid == 0) a.stats[2 * r] = a.stats[2 * r + 1] = a.row_loss[r] = 0.f;
+        if (!ACC) zeros();
+        return;
+    }
+    for (int i = tid; i < (int)(kCols / 32); i += NT) named[i] = 0;
+    if (tid == 0) twice = 0;
+    float4u v[R], low[L ? L : 1];  // the first L pieces go to LDS
+#pragma unroll
+    for (int u = 0; u < L; u++) low[u] = row_piece<true>(x, bytes_from(0, whole), 16 * (tid + u * NT));
+#pragma unroll
+    for (int u = 0; u < R; u++) v[u] = row_piece<true>(x, bytes_from(0, whole), 16 * (tid + (L + u) * NT));
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < L; u++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx = fmaxf(mx, low[u][e]);
+        held[tid + u * NT] = make_float4(low[u].x, low[u].y, low[u].z, low[u].w);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (nothing else finds room in registers before)
+    const float tail = whole + tid < cols ? x[whole + tid] : -INFINITY;
+    // entries tid, tid + NT, ... of the teacher; their columns are counted from the segment's first (others lie behind its end)
+    uint32_t col[kEntries];
+    float t[kEntries], xe[kEntries], f[kEntries], old_e[kEntries];
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < kEntries; i++) {
+        teacher_entry(a, r, tid + i * NT, col[i], t[i]);
+        col[i] = col[i] == kNoCol ? kNoCol : col[i] - first;
+        xe[i] = col[i] < cols ? x[col[i]] : 0.f;
+        top[0] = fmaxf(top[0], t[i]);
+    }
+    float m, ls;
+    if (FWD) {
+#pragma unroll
+        for (int u = 0; u < R; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) mx = fmaxf(mx, v[u][e]);
+        top[1] = fmaxf(tail, mx);
+        row_maxima<NT, 2>(top, smem);
+        m = top[1];
+        ls = 0.f;
+    } else {
+        float one[1] = {top[0]};
+        row_maxima<NT, 1>(one, smem);
+        top[0] = one[0];
+        m = a.stats[2 * r];
+        ls = a.stats[2 * r + 1];
+    }
+    const float from_x = m == -INFINITY ? 0.f : m, from_t = top[0] == -INFINITY ? 0.f : top[0];
+    auto power = [&](float value) { return exp2_fast((value - from_x) * a.scale); };
+    float sum[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kEntries; i++) {
+        float part;
+        teacher_terms(a, t[i], xe[i], from_t, from_x, f[i], part);
+        sum[0] += f[i];
+        sum[1] += part;
+    }
+#pragma unroll
+    for (int u = 0; u < R; u++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[u][e] = power(v[u][e]);
+        sum[2] += (v[u][0] + v[u][1]) + (v[u][2] + v[u][3]);
+    }
+#pragma unroll
+    for (int u = 0; u < L; u++) {
+        float4 h = held[tid + u * NT];
+        h = make_float4(power(h.x), power(h.y), power(h.z), power(h.w));
+        held[tid + u * NT] = h;
+        sum[2] += (h.x + h.y) + (h.z + h.w);
+    }
+    const float tail_e = power(tail);
+    sum[2] += tail_e;
+    float4u old[kBatch];
+    auto load_old = [&](int u0) {
+#pragma unroll
+        for (int u = u0; u < u0 + kBatch && u < R; u++) old[u - u0] = row_piece<true>(grad, bytes_from(0, whole), 16 * (tid + u * NT));
+    };
+    if (ACC) load_old(0);
+    if (FWD) {
+        row_sums<NT, 3>(sum, smem);
+    } else {
+        float one[1] = {sum[0]};
+        row_sums<NT, 1>(one, smem);
+        sum[0] = one[0];
+    }
+    const RowResult res = row_result<FWD>(a, w, m, ls, sum[2], sum[0], sum[1]);
+    if (FWD && tid == 0) {
+        a.stats[2 * r] = res.m;
+        a.stats[2 * r + 1] = res.ls;
+        a.row_loss[r] = res.loss;
+    }
+    if (res.empty) {
+        if (!ACC) zeros();
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kEntries; i++) {
+        const bool here = col[i] < cols;
+        old_e[i] = ACC && here ? grad[col[i]] : 0.f;
+        if (tid + i * NT < kMaxK) {
+            col_of[tid + i * NT] = col[i];
+            q_of[tid + i * NT] = f[i] * res.inv_S;
+        }
+        if (here && (atomicOr(&named[col[i] / 32], 1u << col[i] % 32) >> col[i] % 32 & 1u)) twice = 1;
+    }
+    __syncthreads();  // what is added to has been read where entries stand
+    const float fac = res.f * res.inv_s;  // of a class without a share
+    auto put = [&](uint32_t c, float4u e, float4u add_to) {
+        if (c >= whole) return;
+        float4u g;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float d = e[i] * fac;
+            g[i] = ACC ? add_to[i] + d : d;
+        }
+        __builtin_nontemporal_store(g, reinterpret_cast<float4u*>(grad + c));
+    };
+    if constexpr (ACC) {
+#pragma unroll
+        for (int u0 = 0; u0 < R; u0 += kBatch) {
+            if (u0) load_old(u0);
+#pragma unroll
+            for (int u = u0; u < u0 + kBatch && u < R; u++) put(4 * (tid + u * NT), v[u], old[u - u0]);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < R; u++) put(4 * (tid + (L + u) * NT), v[u], v[u]);
+#pragma unroll
+        for (int u = 0; u < L; u++) {
+            const float4 h = held[tid + u * NT];
+            const float4u e = {h.x, h.y, h.z, h.w};
+            put(4 * (tid + u * NT), e, e);
+        }
+    }
+    if (whole + tid < cols) {
+        const float d = tail_e * fac;
+        grad[whole + tid] = ACC ? grad[whole + tid] + d : d;
+    }
+    // the classes that the teacher names: their shares in the order of j
+    float share[kEntries];
+    bool mine[kEntries];
+#pragma unroll
+    for (int i = 0; i < kEntries; i++) {
+        share[i] = f[i] * res.inv_S;
+        mine[i] = col[i] < cols;
+        if (twice && mine[i]) {
+            share[i] = 0.f;
+            for (uint32_t j = 0; j < a.k; j++) {
+                const bool same = col_of[j] == col[i];
+                if (same && j < (uint32_t)(tid + i * NT)) mine[i] = false;
+                share[i] = same ? share[i] + q_of[j] : share[i];
+            }
+        }
+    }
+    __syncthreads();  // the gradient without shares is written
+#pragma unroll
+    for (int i = 0; i < kEntries; i++)
+        if (mine[i]) {
+            const float d = res.f * (power(xe[i]) * res.inv_s - share[i]);
+            grad[col[i]] = ACC ? old_e[i] + d : d;
+        }
 }
 
 // The loss of rows of any length: a workgroup reads the row with a running maximum per thread, whose sum is rescaled when it grows.
@@ -1175,7 +1355,7 @@ __global__ __launch_bounds__(kStreamNT, 8) void distill_stream_kernel(DistillArg
 static unsigned row_grid(size_t rows) { return (unsigned)(rows < 65536 ? rows : 65536); }
 
 template <bool FWD, bool BWD, bool ACC>
-static int distill_launch(zg_hip_ctx* ctx, const DistillArgs& a, float* loss, bool* summed) {
+static int distill_launch(zg_hip_ctx* ctx, DistillArgs a, float* loss, bool* summed) {
     *summed = false;
     if (a.cols <= 256 && a.k <= 16) {
         const size_t blocks = ceil_div_sz(a.rows, 16);
@@ -1195,23 +1375,40 @@ static int distill_launch(zg_hip_ctx* ctx, const DistillArgs& a, float* loss, bo
         ZG_LAUNCH_CHECK();
         return ZG_HIP_OK;
     }
-#define ZG_ROWS(NT, VPT, UP)                                                                                                          \
-    hipLaunchKernelGGL((distill_row_kernel<NT, VPT, UP, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(a.rows * segments, NT < 256 ? 256 / NT : 1)), \
+#define ZG_ROWS(NT, VPT)                                                                                                        \
+    hipLaunchKernelGGL((distill_row_kernel<NT, VPT, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(a.rows, NT < 256 ? 256 / NT : 1)), \
                        dim3(NT < 256 ? 256 : NT), 0, ctx->stream, a)
-    // a gradient that finds its statistics takes long rows segment by segment
-    const size_t segments = FWD || a.cols <= 2048 ? 1 : ceil_div_sz(a.cols, 8192);
-    ZG_REQUIRE(a.rows * segments < 0x7fffffffull, "distill: %zu rows of %u columns", a.rows, a.cols);
+#define ZG_GRAD(NT, R, L) \
+    hipLaunchKernelGGL((distill_grad_kernel<NT, R, L, FWD, ACC>), dim3((unsigned)(a.rows * a.segments)), dim3(NT), 0, ctx->stream, a)
+    // (the gradient alone: even segments)
+    a.segments = FWD || a.cols <= 8192 ? 1u : (a.cols - 1) / 8192 + 1;
+    a.segment = ((a.cols - 1) / a.segments + 4) & ~3u;
+    a.segments = (a.cols - 1) / a.segment + 1;  // as many as have columns
+    ZG_REQUIRE(a.rows * a.segments < 0x7fffffffull, "distill: %zu rows of %u columns", a.rows, a.cols);
     if (a.cols <= 1024) {
-        ZG_ROWS(64, 4, 4);
+        ZG_ROWS(64, 4);
     } else if (a.cols <= 2048) {
-        ZG_ROWS(64, 8, 8);
-    } else if (!FWD || a.cols <= 8192) {
-        ZG_ROWS(256, 8, 4);
-    } else if constexpr (FWD && BWD) {
-        if (a.cols <= 32768) {
-            ZG_ROWS(1024, 8, 2);
+        ZG_ROWS(64, 8);
+    } else if constexpr (!BWD) {
+        if (a.cols <= 4096) ZG_ROWS(256, 4);
+        else if (a.cols <= 8192) ZG_ROWS(256, 8);
+        else if (a.cols <= 16384) ZG_ROWS(1024, 4);
+        else if (a.cols <= 32768) ZG_ROWS(1024, 8);
+        else hipLaunchKernelGGL(distill_stream_kernel, dim3(row_grid(a.rows)), dim3(kStreamNT), 0, ctx->stream, a);
+    } else if (a.segment <= 4096) {
+        ZG_GRAD(256, 4, 0);
+    } else if (a.segment <= 8192) {
+        ZG_GRAD(256, 8, 0);
+    } else if constexpr (FWD) {
+        if (a.cols <= 16384) {
+            ZG_GRAD(1024, 4, 0);
+        } else if (a.cols <= 32768) {
+            ZG_GRAD(1024, 8, 0);
+        } else if (a.cols <= 53248) {
+            if constexpr (ACC) ZG_GRAD(1024, 13, 0);
+            else ZG_GRAD(1024, 9, 4);
         } else if (a.cols <= 65536) {
-            ZG_ROWS(1024, 16, 2);
+            ZG_GRAD(1024, 16, 0);
         } else {
             // Rows that no workgroup holds: the loss, then the gradient.  (2048 x 128000: 560 us, one kernel that read each row twice
             // 526; 16 x 128000: 23 us against 36.  Some rows at a time, for the second pass to find them in the memory-side cache,
@@ -1220,10 +1417,8 @@ static int distill_launch(zg_hip_ctx* ctx, const DistillArgs& a, float* loss, bo
             if (int rc = distill_launch<true, false, false>(ctx, a, loss, &unused)) return rc;
             return distill_launch<false, true, ACC>(ctx, a, loss, &unused);
         }
-    } else if constexpr (FWD) {
-        if (a.cols <= 32768) ZG_ROWS(1024, 8, 2);
-        else hipLaunchKernelGGL(distill_stream_kernel, dim3(row_grid(a.rows)), dim3(kStreamNT), 0, ctx->stream, a);
     }
+#undef ZG_GRAD
 #undef ZG_ROWS
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
@@ -1389,7 +1584,7 @@ static int distill_entry(zg_hip_ctx* ctx, const char* op, const float* logits, c
     DeviceGuard guard(ctx);
     const float inv_temp = 1.f / temperature;
     DistillArgs a{logits, teacher, indices, row_weights, stats, row_loss, grad, rows, (uint32_t)cols, (uint32_t)k, temperature, inv_temp,
-                  inv_temp * 1.44269504088896340736f, 1.f / (float)rows};
+                  inv_temp * 1.44269504088896340736f, 1.f / (float)rows, 1, (uint32_t)cols};
     bool summed = false;
     int rc;
     if (fwd && !bwd) rc = distill_launch<true, false, false>(ctx, a, loss, &summed);
