@@ -86,12 +86,32 @@ struct Place {
 // there.  Pieces behind that are -inf, which loses to every value of the row: a buffer load takes any 4-byte alignment and
 // reads nothing behind the end.
 typedef unsigned uint4v __attribute__((ext_vector_type(4)));
-template <bool ONCE = false>  // ONCE: nothing will read it again soon
+template <bool ONCE = false>  // ONCE: past the memory-side cache
 __device__ __forceinline__ float4u row_piece(const float* base, uint32_t bytes, uint32_t off) {
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, (int)bytes, 0x00020000);
     const float4u v = __builtin_bit_cast(float4u, (uint4v)__builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, ONCE ? 2 : 0));
     const bool in = off < bytes;
     return float4u{in ? v.x : -INFINITY, in ? v.y : -INFINITY, in ? v.z : -INFINITY, in ? v.w : -INFINITY};
+}
+// N pieces of a row, `by` bytes apart; all loads before the first is waited for
+template <int N>
+__device__ __forceinline__ void row_pieces(float4u* v, const float* base, uint32_t bytes, uint32_t off, uint32_t by, bool once) {
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, (int)bytes, 0x00020000);
+    uint4v raw[N];
+    if (once) {
+#pragma unroll
+        for (int u = 0; u < N; u++) raw[u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(off + u * by), 0, 2);
+    } else {
+#pragma unroll
+        for (int u = 0; u < N; u++) raw[u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(off + u * by), 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+        const float4u p = __builtin_bit_cast(float4u, raw[u]);
+        const bool in = off + u * by < bytes;
+        v[u] = float4u{in ? p.x : -INFINITY, in ? p.y : -INFINITY, in ? p.z : -INFINITY, in ? p.w : -INFINITY};
+    }
 }
 __device__ __forceinline__ uint32_t bytes_from(uint32_t c0, uint32_t whole) {  // whole: columns in whole pieces
     const uint32_t left = c0 < whole ? whole - c0 : 0u;
@@ -742,7 +762,13 @@ struct DistillArgs {
     uint32_t cols, k;
     float temp, inv_temp, scale, mean;  // scale = log2(e) / temp
     uint32_t segments, segment;         // the gradient alone: parts of a row, and their columns
+    bool once;                          // more is read than the memory-side cache holds: loads leave nothing there
 };
+
+// Loads that pass by the memory-side cache (256 MB) win as soon as it can not hold what is read (logits, an old gradient: 16384 x
+// 10001 forward 171 -> 109 us, 8192 x 32000 168 -> 159; 8000 x 8000 added to the gradient 149 -> 131) and lose before (1000 x
+// 50257 step 71 -> 85 us, 5000 x 10000 70 -> 77); in between both take the same (1500 x 50257: step 118 and 124, forward 61 and 60).
+constexpr size_t kCachedFloats = (size_t)80 << 20;
 
 // the hardware's 2^x: off by a step at most, which with the roundings of its argument is what exp(x) of a library has lost as well
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -994,8 +1020,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 ? 8 : 1) void disti
         return;
     }
     float4u v[VPT];
-#pragma unroll
-    for (int u = 0; u < VPT; u++) v[u] = row_piece(x, bytes_from(0, whole), 16 * (tid + u * NT));
+    row_pieces<VPT>(v, x, bytes_from(0, whole), 16 * tid, 16 * NT, a.once);
     const float tail = whole + tid < cols ? x[whole + tid] : -INFINITY;  // of the first threads
     uint32_t col[kEntries];
     float t[kEntries], xe[kEntries];
@@ -1107,7 +1132,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 ? 8 : 1) void disti
 // Rows of 32769 to 53248 columns fit twice on a compute unit that way, so that one is read or written while the other is summed
 // up.  (2048 x 50257, k = 100: 165 us against 189 with the row in registers and shares from LDS; 8192 x 32000: 355 against 394; added
 // to an old gradient, whose pieces take the registers: 221 against 250 and 496 against 581.)
-template <int NT, int R, int L, bool FWD, bool ACC>
+template <int NT, int R, int L, bool FWD, bool ACC, bool ONCE>
 __global__ __launch_bounds__(NT, R <= (ACC ? 4 : 9) ? 8 : 4) void distill_grad_kernel(DistillArgs a) {
     static_assert(!ACC || L == 0, "old pieces of those in LDS");
     constexpr uint32_t kCols = 4 * NT * (R + L);
@@ -1139,9 +1164,9 @@ __global__ __launch_bounds__(NT, R <= (ACC ? 4 : 9) ? 8 : 4) void distill_grad_k
     if (tid == 0) twice = 0;
     float4u v[R], low[L ? L : 1];  // the first L pieces go to LDS
 #pragma unroll
-    for (int u = 0; u < L; u++) low[u] = row_piece<true>(x, bytes_from(0, whole), 16 * (tid + u * NT));
+    for (int u = 0; u < L; u++) low[u] = row_piece<ONCE>(x, bytes_from(0, whole), 16 * (tid + u * NT));
 #pragma unroll
-    for (int u = 0; u < R; u++) v[u] = row_piece<true>(x, bytes_from(0, whole), 16 * (tid + (L + u) * NT));
+    for (int u = 0; u < R; u++) v[u] = row_piece<ONCE>(x, bytes_from(0, whole), 16 * (tid + (L + u) * NT));
     float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < L; u++) {
@@ -1207,7 +1232,7 @@ __global__ __launch_bounds__(NT, R <= (ACC ? 4 : 9) ? 8 : 4) void distill_grad_k
     float4u old[kBatch];
     auto load_old = [&](int u0) {
 #pragma unroll
-        for (int u = u0; u < u0 + kBatch && u < R; u++) old[u - u0] = row_piece<true>(grad, bytes_from(0, whole), 16 * (tid + u * NT));
+        for (int u = u0; u < u0 + kBatch && u < R; u++) old[u - u0] = row_piece<ONCE>(grad, bytes_from(0, whole), 16 * (tid + u * NT));
     };
     if (ACC) load_old(0);
     if (FWD) {
@@ -1317,8 +1342,7 @@ __global__ __launch_bounds__(kStreamNT, 8) void distill_stream_kernel(DistillArg
         float mine = -INFINITY, s = 0.f;  // this thread's maximum, and its sum from there
         for (uint32_t c0 = 0; c0 < whole; c0 += 4 * NT * U) {
             float4u v[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) v[u] = row_piece(x + c0, bytes_from(c0, whole), 16 * (tid + u * NT));
+            row_pieces<U>(v, x + c0, bytes_from(c0, whole), 16 * tid, 16 * NT, a.once);
             float mx = v[0][0];
 #pragma unroll
             for (int u = 0; u < U; u++)
@@ -1378,8 +1402,12 @@ static int distill_launch(zg_hip_ctx* ctx, DistillArgs a, float* loss, bool* sum
 #define ZG_ROWS(NT, VPT)                                                                                                        \
     hipLaunchKernelGGL((distill_row_kernel<NT, VPT, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(a.rows, NT < 256 ? 256 / NT : 1)), \
                        dim3(NT < 256 ? 256 : NT), 0, ctx->stream, a)
-#define ZG_GRAD(NT, R, L) \
-    hipLaunchKernelGGL((distill_grad_kernel<NT, R, L, FWD, ACC>), dim3((unsigned)(a.rows * a.segments)), dim3(NT), 0, ctx->stream, a)
+#define ZG_GRAD(NT, R, L)                                                                                                              \
+    do {                                                                                                                               \
+        const dim3 grid((unsigned)(a.rows * a.segments));                                                                              \
+        if (a.once) hipLaunchKernelGGL((distill_grad_kernel<NT, R, L, FWD, ACC, true>), grid, dim3(NT), 0, ctx->stream, a);            \
+        else hipLaunchKernelGGL((distill_grad_kernel<NT, R, L, FWD, ACC, false>), grid, dim3(NT), 0, ctx->stream, a);                  \
+    } while (0)
     // (the gradient alone: even segments)
     a.segments = FWD || a.cols <= 8192 ? 1u : (a.cols - 1) / 8192 + 1;
     a.segment = ((a.cols - 1) / a.segments + 4) & ~3u;
@@ -1390,9 +1418,9 @@ static int distill_launch(zg_hip_ctx* ctx, DistillArgs a, float* loss, bool* sum
     } else if (a.cols <= 2048) {
         ZG_ROWS(64, 8);
     } else if constexpr (!BWD) {
-        if (a.cols <= 4096) ZG_ROWS(256, 4);
+        if (a.cols <= 4096) ZG_ROWS(64, 16);
         else if (a.cols <= 8192) ZG_ROWS(256, 8);
-        else if (a.cols <= 16384) ZG_ROWS(1024, 4);
+        else if (a.cols <= 16384) ZG_ROWS(512, 8);
         else if (a.cols <= 32768) ZG_ROWS(1024, 8);
         else hipLaunchKernelGGL(distill_stream_kernel, dim3(row_grid(a.rows)), dim3(kStreamNT), 0, ctx->stream, a);
     } else if (a.segment <= 4096) {
@@ -1584,7 +1612,8 @@ static int distill_entry(zg_hip_ctx* ctx, const char* op, const float* logits, c
     DeviceGuard guard(ctx);
     const float inv_temp = 1.f / temperature;
     DistillArgs a{logits, teacher, indices, row_weights, stats, row_loss, grad, rows, (uint32_t)cols, (uint32_t)k, temperature, inv_temp,
-                  inv_temp * 1.44269504088896340736f, 1.f / (float)rows, 1, (uint32_t)cols};
+                  inv_temp * 1.44269504088896340736f, 1.f / (float)rows, 1, (uint32_t)cols,
+                  rows * cols * (accumulate ? 2 : 1) > kCachedFloats};
     bool summed = false;
     int rc;
     if (fwd && !bwd) rc = distill_launch<true, false, false>(ctx, a, loss, &summed);
