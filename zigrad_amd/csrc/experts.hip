@@ -134,16 +134,20 @@ __global__ __launch_bounds__(kSortThreads) void expert_place_kernel(const uint64
 // ------------------------------------------------------------------------------------------------
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
+template <bool ONCE = false>  // ONCE: past the memory-side cache
 __device__ __forceinline__ float4u load_piece(const float* row, size_t c, size_t width) {
+    if (ONCE && c + 4 <= width) return __builtin_nontemporal_load(reinterpret_cast<const float4u*>(row + c));
     if (c + 4 <= width) return *reinterpret_cast<const float4u*>(row + c);
     float4u v = {row[c], 0.f, 0.f, 0.f};
     if (c + 1 < width) v.y = row[c + 1];
     if (c + 2 < width) v.z = row[c + 2];
     return v;
 }
+template <bool ONCE = false>
 __device__ __forceinline__ void store_piece(float* row, size_t c, size_t width, float4u v) {
     if (c + 4 <= width) {
-        *reinterpret_cast<float4u*>(row + c) = v;
+        if (ONCE) __builtin_nontemporal_store(v, reinterpret_cast<float4u*>(row + c));
+        else *reinterpret_cast<float4u*>(row + c) = v;
         return;
     }
     row[c] = v.x;
@@ -164,6 +168,7 @@ __device__ __forceinline__ void split(size_t i, size_t by, size_t& q, size_t& re
 
 constexpr int kEntriesAtOnce = 4;  // of a token, whose loads are in flight together
 
+template <bool ONCE>
 __global__ __launch_bounds__(kBlock) void expert_spread_kernel(const float* x, const uint64_t* slots, float* y, size_t n_tokens,
                                                                 size_t k, size_t width) {
     const size_t pieces = (width + 3) / 4, total = n_tokens * pieces, places = n_tokens * k;
@@ -177,13 +182,13 @@ __global__ __launch_bounds__(kBlock) void expert_spread_kernel(const float* x, c
             for (int u = 0; u < kEntriesAtOnce; u++) s[u] = j0 + u < k ? slots[t * k + j0 + u] : ~(uint64_t)0;
 #pragma unroll
             for (int u = 0; u < kEntriesAtOnce; u++)
-                if (s[u] < places) store_piece(y + s[u] * width, 4 * p, width, v);
+                if (s[u] < places) store_piece<ONCE>(y + s[u] * width, 4 * p, width, v);
         }
     }
 }
 
 // SCALE: the weighted sum; else the plain one.  ACC: added to what is there.
-template <bool SCALE, bool ACC>
+template <bool SCALE, bool ACC, bool ONCE>
 __global__ __launch_bounds__(kBlock) void expert_gather_kernel(const float* y, const uint64_t* slots, const float* weights,
                                                                 float* out, size_t n_tokens, size_t k, size_t width) {
     const size_t pieces = (width + 3) / 4, total = n_tokens * pieces, places = n_tokens * k;
@@ -202,7 +207,7 @@ __global__ __launch_bounds__(kBlock) void expert_gather_kernel(const float* y, c
                 held[u] = s < places;
                 w[u] = SCALE && held[u] ? weights[t * k + j0 + u] : 1.f;
                 v[u] = float4u{0.f, 0.f, 0.f, 0.f};
-                if (held[u]) v[u] = load_piece(y + s * width, 4 * p, width);
+                if (held[u]) v[u] = load_piece<ONCE>(y + s * width, 4 * p, width);
             }
 #pragma unroll
             for (int u = 0; u < kEntriesAtOnce; u++)
@@ -218,7 +223,8 @@ __global__ __launch_bounds__(kBlock) void expert_gather_kernel(const float* y, c
 
 // The backward of the combination: L lanes take an entry, scale its token's gradient into its row and sum up the product of that gradient
 // with the entry's output in the same pass.  ROWS / WEIGHTS: which of the two are wanted.
-template <int L, bool ROWS, bool WEIGHTS>
+// ONCE_IN, ONCE_OUT: y and y_g pass by the memory-side cache.
+template <int L, bool ROWS, bool WEIGHTS, bool ONCE_IN, bool ONCE_OUT>
 __global__ __launch_bounds__(kBlock) void expert_combine_bwd_kernel(const float* out_g, const float* y, const uint64_t* slots,
                                                                      const float* weights, float* y_g, float* weights_g,
                                                                      size_t n_tokens, size_t k, size_t width) {
@@ -242,7 +248,7 @@ __global__ __launch_bounds__(kBlock) void expert_combine_bwd_kernel(const float*
                     g[u] = v[u] = float4u{0.f, 0.f, 0.f, 0.f};
                     if (p < pieces) {
                         g[u] = load_piece(g_row, 4 * p, width);
-                        if (WEIGHTS) v[u] = load_piece(y_row, 4 * p, width);
+                        if (WEIGHTS) v[u] = load_piece<ONCE_IN>(y_row, 4 * p, width);
                     }
                 }
 #pragma unroll
@@ -250,7 +256,7 @@ __global__ __launch_bounds__(kBlock) void expert_combine_bwd_kernel(const float*
                     const size_t p = p0 + (size_t)u * L;
                     if (WEIGHTS) sum += (g[u].x * v[u].x + g[u].y * v[u].y) + (g[u].z * v[u].z + g[u].w * v[u].w);
                     if (ROWS && p < pieces)
-                        store_piece(y_g + s * width, 4 * p, width, float4u{w * g[u].x, w * g[u].y, w * g[u].z, w * g[u].w});
+                        store_piece<ONCE_OUT>(y_g + s * width, 4 * p, width, float4u{w * g[u].x, w * g[u].y, w * g[u].z, w * g[u].w});
                 }
             }
         }
@@ -266,6 +272,11 @@ static unsigned flat_grid(size_t items) {
     const size_t b = ceil_div_sz(items, kBlock);
     return (unsigned)(b < 1048576 ? b : 1048576);
 }
+// Whether so many floats pass a kernel once that the memory-side cache (256 MB) can not hold them.  Loads and stores that pass by it win
+// then (8 entries of width 1024 for 16384 tokens: dispatch 110 -> 101 us, combine 117 -> 106, combine_bwd 217 -> 198; for 8192 tokens
+// dispatch 58 -> 51 and combine_bwd, whose stores still go to the cache, 110 -> 98) and lose before (6 of 1030 for 4095: combine 21 -> 27,
+// combine_bwd 39 -> 45).
+static bool past_cache(size_t floats) { return floats > (size_t)64 << 20; }
 static int experts_check(const char* op, const uint64_t* slots, size_t n_tokens, size_t k, size_t width) {
     ZG_REQUIRE(k >= 1 && k <= ZG_HIP_EXPERTS_MAX_K, "%s: k = %zu is not in 1 .. %d", op, k, (int)ZG_HIP_EXPERTS_MAX_K);
     ZG_REQUIRE(mul_sat(mul_sat(n_tokens, k), width) < ((size_t)1 << 60), "%s: %zu x %zu rows of %zu", op, n_tokens, k, width);
@@ -321,7 +332,11 @@ ZG_API int zg_hip_expert_dispatch(zg_hip_ctx* ctx, const float* x, const uint64_
     ZG_REQUIRE(!ranges_overlap(y, bytes, x, n_tokens * width * 4) && !ranges_overlap(y, bytes, slots, n_tokens * k * 8),
                "expert_dispatch: y overlaps an input");
     DeviceGuard guard(ctx);
-    hipLaunchKernelGGL(expert_spread_kernel, dim3(flat_grid(n_tokens * ((width + 3) / 4))), dim3(kBlock), 0, ctx->stream, x, slots, y,
+    if (past_cache(n_tokens * width * k + n_tokens * width))
+        hipLaunchKernelGGL(expert_spread_kernel<true>, dim3(flat_grid(n_tokens * ((width + 3) / 4))), dim3(kBlock), 0, ctx->stream, x, slots, y,
+                       n_tokens, k, width);
+    else
+        hipLaunchKernelGGL(expert_spread_kernel<false>, dim3(flat_grid(n_tokens * ((width + 3) / 4))), dim3(kBlock), 0, ctx->stream, x, slots, y,
                        n_tokens, k, width);
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
@@ -331,7 +346,11 @@ namespace zg {
 template <bool SCALE, bool ACC>
 static int launch_gather(zg_hip_ctx* ctx, const float* y, const uint64_t* slots, const float* weights, float* out, size_t n_tokens,
                          size_t k, size_t width) {
-    hipLaunchKernelGGL((expert_gather_kernel<SCALE, ACC>), dim3(flat_grid(n_tokens * ((width + 3) / 4))), dim3(kBlock), 0, ctx->stream, y,
+    if (past_cache(n_tokens * width * k + n_tokens * width))
+        hipLaunchKernelGGL((expert_gather_kernel<SCALE, ACC, true>), dim3(flat_grid(n_tokens * ((width + 3) / 4))), dim3(kBlock), 0, ctx->stream, y,
+                       slots, weights, out, n_tokens, k, width);
+    else
+        hipLaunchKernelGGL((expert_gather_kernel<SCALE, ACC, false>), dim3(flat_grid(n_tokens * ((width + 3) / 4))), dim3(kBlock), 0, ctx->stream, y,
                        slots, weights, out, n_tokens, k, width);
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
@@ -383,9 +402,17 @@ ZG_API int zg_hip_expert_combine_bwd(zg_hip_ctx* ctx, const float* out_g, const 
     DeviceGuard guard(ctx);
     if (!y_g && !weights_g) return ZG_HIP_OK;
     // 16 lanes an entry for narrow rows, a wave else
-#define ZG_COMBINE_BWD(L, ROWS, WEIGHTS)                                                                                            \
-    hipLaunchKernelGGL((expert_combine_bwd_kernel<L, ROWS, WEIGHTS>), dim3(flat_grid(n * (L))), dim3(kBlock), 0, ctx->stream, out_g, y, \
-                       slots, weights, y_g, weights_g, n_tokens, k, width)
+    const bool once_in = past_cache(n * width * ((y_g ? 1 : 0) + (weights_g ? 1 : 0)) + n_tokens * width);
+    const bool once_out = past_cache(n * width);
+#define ZG_COMBINE_BWD_(L, ROWS, WEIGHTS, IN, OUT)                                                                                     \
+    hipLaunchKernelGGL((expert_combine_bwd_kernel<L, ROWS, WEIGHTS, IN, OUT>), dim3(flat_grid(n * (L))), dim3(kBlock), 0, ctx->stream, \
+                       out_g, y, slots, weights, y_g, weights_g, n_tokens, k, width)
+#define ZG_COMBINE_BWD(L, ROWS, WEIGHTS)                                                       \
+    do {                                                                                       \
+        if (ROWS && once_out) ZG_COMBINE_BWD_(L, ROWS, WEIGHTS, WEIGHTS, ROWS);                \
+        else if (WEIGHTS && once_in) ZG_COMBINE_BWD_(L, ROWS, WEIGHTS, WEIGHTS, false);        \
+        else ZG_COMBINE_BWD_(L, ROWS, WEIGHTS, false, false);                                  \
+    } while (0)
     if (width <= 128) {
         if (y_g && weights_g) ZG_COMBINE_BWD(16, true, true);
         else if (y_g) ZG_COMBINE_BWD(16, true, false);
@@ -396,6 +423,7 @@ ZG_API int zg_hip_expert_combine_bwd(zg_hip_ctx* ctx, const float* out_g, const 
         else ZG_COMBINE_BWD(64, false, true);
     }
 #undef ZG_COMBINE_BWD
+#undef ZG_COMBINE_BWD_
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
 }
