@@ -40,14 +40,14 @@ constexpr int kMaxK = ZG_HIP_TOPK_MAX_K;
 // ------------------------------------------------------------------------------------------------
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes at any 4-byte alignment
 
-constexpr uint32_t kSegment = 1024;  // candidates a wave has room for
+constexpr int kSegment = 1024;       // candidates a wave has room for, or fewer (SEG)
 constexpr uint32_t kRankMost = 384;
 constexpr int kThin = 6;             // times 64: candidates of a wave that are thinned out with ballots
 
-template <int NT>
+template <int NT, int SEG = kSegment>
 struct Select {
     static constexpr int kWaves = NT / kWave;
-    uint64_t key[kWaves][kSegment + 2];
+    uint64_t key[kWaves][SEG + 2];
     uint32_t hist[256];
     uint32_t low[kWaves];       // the waves' bounds
     uint32_t n[kWaves];         // candidates, written down where other waves need them
@@ -122,31 +122,31 @@ __device__ __forceinline__ uint32_t lanes_below(uint64_t lanes) {  // how many o
 }
 
 // Those of the four values that reach the bound become candidates of the wave, all of whose lanes call this.  Candidates past
-// kSegment are counted and find no room.  CHECK: columns from `cols` on are none.
-template <int NT, bool CHECK>
-__device__ __forceinline__ void push_piece(Select<NT>& s, Place& at, float4u v, uint32_t col, uint32_t cols, float low) {
+// SEG are counted and find no room.  CHECK: columns from `cols` on are none.
+template <int NT, bool CHECK, int SEG>
+__device__ __forceinline__ void push_piece(Select<NT, SEG>& s, Place& at, float4u v, uint32_t col, uint32_t cols, float low) {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const bool in = !(v[e] < low) && (!CHECK || col + e < cols);
         const uint64_t ins = __ballot(in);
         if (!ins) continue;
         const uint32_t to = at.n + lanes_below(ins);
-        if (in && to < kSegment) s.key[at.wave][to] = ((uint64_t)__float_as_uint(v[e]) << 32) | (col + e);
+        if (in && to < SEG) s.key[at.wave][to] = ((uint64_t)__float_as_uint(v[e]) << 32) | (col + e);
         at.n += (uint32_t)__popcll(ins);
     }
     __builtin_amdgcn_sched_barrier(0);  // a piece at a time: done side by side they cost the registers of half the waves
 }
 // The up to three values behind the row's whole pieces.
-template <int NT>
-__device__ __forceinline__ void push_tail(Select<NT>& s, Place& at, const float* row, uint32_t whole, uint32_t cols, float low) {
+template <int NT, int SEG>
+__device__ __forceinline__ void push_tail(Select<NT, SEG>& s, Place& at, const float* row, uint32_t whole, uint32_t cols, float low) {
     if (whole == cols || at.wave != 0) return;
     const uint32_t col = whole + at.lane;
     const float x = col < cols ? row[col] : -INFINITY;
     push_piece<NT, true>(s, at, float4u{x, -INFINITY, -INFINITY, -INFINITY}, col, col < cols ? col + 1 : 0u, low);
 }
 // The candidates that came since are turned into keys.
-template <int NT>
-__device__ __forceinline__ void key_candidates(Select<NT>& s, Place& at) {
+template <int NT, int SEG>
+__device__ __forceinline__ void key_candidates(Select<NT, SEG>& s, Place& at) {
     select_sync<kWave>();
     for (uint32_t i = at.keyed + at.lane; i < at.n; i += kWave) {
         const uint64_t c = s.key[at.wave][i];
@@ -156,8 +156,8 @@ __device__ __forceinline__ void key_candidates(Select<NT>& s, Place& at) {
 }
 
 // The most candidates any wave has; a sync.
-template <int NT>
-__device__ __forceinline__ uint32_t select_most(Select<NT>& s, const Place& at) {
+template <int NT, int SEG>
+__device__ __forceinline__ uint32_t select_most(Select<NT, SEG>& s, const Place& at) {
     if constexpr (NT == kWave) {
         select_sync<NT>();
         return at.n;
@@ -173,8 +173,8 @@ __device__ __forceinline__ uint32_t select_most(Select<NT>& s, const Place& at) 
 
 // Leaves the k largest of the candidates (none lost, at least k) and returns the bound for values of later columns.  All threads
 // call it after select_most.
-template <int NT>
-__device__ Bound select_cut(Select<NT>& s, Place& at, uint32_t k) {
+template <int NT, int SEG>
+__device__ Bound select_cut(Select<NT, SEG>& s, Place& at, uint32_t k) {
     const int lane = at.lane;
     key_candidates<NT>(s, at);
     uint64_t prefix = 0, mask = 0;
@@ -242,7 +242,7 @@ __device__ Bound select_cut(Select<NT>& s, Place& at, uint32_t k) {
 template <int KEYS>
 __device__ __forceinline__ uint32_t wave_bound(const uint32_t (&key)[KEYS], uint32_t share) {
     uint32_t t = 0;
-#pragma unroll 1
+#pragma unroll
     for (int bit = 31; bit >= 16; bit--) {
         const uint32_t c = t | (1u << bit);
         uint32_t reach = 0;
@@ -254,8 +254,8 @@ __device__ __forceinline__ uint32_t wave_bound(const uint32_t (&key)[KEYS], uint
     return t;
 }
 // The lowest of the waves' bounds: k values of the row reach it when each wave bounds its share of k.
-template <int NT>
-__device__ __forceinline__ uint32_t lowest_bound(Select<NT>& s, const Place& at, uint32_t t) {
+template <int NT, int SEG>
+__device__ __forceinline__ uint32_t lowest_bound(Select<NT, SEG>& s, const Place& at, uint32_t t) {
     if constexpr (NT != kWave) {
         if (at.lane == 0) s.low[at.wave] = t;
         __syncthreads();
@@ -267,8 +267,8 @@ __device__ __forceinline__ uint32_t lowest_bound(Select<NT>& s, const Place& at,
 
 // Drops candidates that a bound from the candidates themselves excludes (a few hundred come down to little more than k; ranking is
 // quadratic in what is left) and returns that bound.  No wave has more than 64 KEYS; all threads call it after a sync.
-template <int NT, int KEYS>
-__device__ __forceinline__ uint32_t select_thin(Select<NT>& s, Place& at, uint32_t share) {
+template <int NT, int KEYS, int SEG>
+__device__ __forceinline__ uint32_t select_thin(Select<NT, SEG>& s, Place& at, uint32_t share) {
     key_candidates<NT>(s, at);
     select_sync<kWave>();
     uint32_t key[KEYS];
@@ -296,13 +296,13 @@ __device__ __forceinline__ uint32_t select_thin(Select<NT>& s, Place& at, uint32
 }
 
 // The row again, NT x 4 values at a time, with room made before each.
-template <int NT>
-__device__ void select_slowly(Select<NT>& s, Place& at, const float* row, uint32_t cols, uint32_t k) {
+template <int NT, int SEG>
+__device__ void select_slowly(Select<NT, SEG>& s, Place& at, const float* row, uint32_t cols, uint32_t k) {
     const uint32_t whole = cols & ~3u;
     Bound bound = bound_of(0u);
     at.n = at.keyed = 0;
     for (uint32_t c0 = 0; c0 < cols; c0 += 4 * NT) {  // (the last round may hold nothing but the tail)
-        if (select_most<NT>(s, at) > kSegment - 5 * kWave) bound = select_cut<NT>(s, at, k);
+        if (select_most<NT>(s, at) > SEG - 5 * kWave) bound = select_cut<NT>(s, at, k);
         push_piece<NT, true>(s, at, row_piece(row + c0, bytes_from(c0, whole), 16 * at.tid), c0 + 4 * at.tid, whole, bound.low);
         if (cols - c0 <= 4 * NT) push_tail<NT>(s, at, row, whole, cols, bound.low);
         select_sync<NT>();
@@ -319,8 +319,8 @@ __device__ __forceinline__ void load_tile(float4u (&v)[VPT], const Place& at, co
         v[u] = BEYOND ? __builtin_nontemporal_load(reinterpret_cast<const float4u*>(row) + at.tid + u * NT)
                       : row_piece(row, bytes_from(0, cols & ~3u), 16 * (at.tid + u * NT));
 }
-template <int NT, int VPT, int U, bool BEYOND>
-__device__ __forceinline__ void select_row(Select<NT>& s, Place& at, float4u (&v)[VPT], const float* row, const float* next,
+template <int NT, int VPT, int U, bool BEYOND, int SEG>
+__device__ __forceinline__ void select_row(Select<NT, SEG>& s, Place& at, float4u (&v)[VPT], const float* row, const float* next,
                                            uint32_t cols, uint32_t k) {
     constexpr uint32_t kTile = 4 * NT * VPT;
     constexpr uint32_t kStep = 4 * NT * U;  // columns of the pieces that are looked through or on their way at a time
@@ -337,12 +337,17 @@ __device__ __forceinline__ void select_row(Select<NT>& s, Place& at, float4u (&v
     for (int u = 1; u < VPT; u++)
 #pragma unroll
         for (int e = 0; e < 4; e++) top[e] = larger(top[e], v[u][e]);
-    uint32_t group[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) group[e] = order_key(top[e]);
     // each wave bounds its share of k by its own groups, without waiting for the others
     const uint32_t share = (k + Select<NT>::kWaves - 1) / Select<NT>::kWaves;
-    Bound bound = bound_of(lowest_bound<NT>(s, at, wave_bound<4>(group, share)));
+    uint32_t t;
+    if (share <= 32) {  // 64 groups do for a small share, a quarter of the counting
+        const uint32_t one[1] = {order_key(larger(larger(top[0], top[1]), larger(top[2], top[3])))};
+        t = wave_bound<1>(one, share);
+    } else {
+        const uint32_t four[4] = {order_key(top[0]), order_key(top[1]), order_key(top[2]), order_key(top[3])};
+        t = wave_bound<4>(four, share);
+    }
+    Bound bound = bound_of(lowest_bound<NT>(s, at, t));
     at.n = at.keyed = 0;
 #pragma unroll
     for (int u = 0; u < VPT; u++) push_piece<NT, !BEYOND>(s, at, v[u], 4 * (at.tid + u * NT), whole, bound.low);
@@ -355,7 +360,7 @@ __device__ __forceinline__ void select_row(Select<NT>& s, Place& at, float4u (&v
         auto look = [&]() {
             if constexpr (NT == kWave) {
                 if (at.n <= 2 * k + kWave) return;
-                room = at.n <= kSegment;
+                room = at.n <= SEG;
                 if (!room) return;
                 Bound b;
                 if (at.n <= kThin * kWave) b = bound_of(select_thin<NT, kThin>(s, at, k));
@@ -363,9 +368,9 @@ __device__ __forceinline__ void select_row(Select<NT>& s, Place& at, float4u (&v
                 if (b.key > bound.key) bound = b;
             } else if ((c0 - kTile) % (4 * kStep) == 0) {
                 const uint32_t most = select_most<NT>(s, at);
-                room = most <= kSegment;
+                room = most <= SEG;
                 if (!room) return;
-                if (most > kSegment / 2) {
+                if (most > SEG / 2) {
                     const Bound b = select_cut<NT>(s, at, k);
                     if (b.key > bound.key) bound = b;
                 }
@@ -401,16 +406,70 @@ __device__ __forceinline__ void select_row(Select<NT>& s, Place& at, float4u (&v
         }
     }
     if (next) load_tile<NT, VPT, BEYOND>(v, at, next, cols);
-    if (select_most<NT>(s, at) > kSegment) {
+    if (select_most<NT>(s, at) > SEG) {
         select_sync<NT>();
         select_slowly<NT>(s, at, row, cols, k);
     }
     key_candidates<NT>(s, at);
 }
 
-// The k largest candidates in order, by rank: emit(rank, key).
-template <int NT, class Emit>
-__device__ __forceinline__ void select_emit(Select<NT>& s, Place& at, uint32_t k, Emit emit) {
+// The value of the lane whose number differs in the bits of M.
+template <int M>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    if constexpr (M == 1) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
+    else if constexpr (M == 2) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+    else if constexpr (M == 8) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true);  // row_ror 8
+    else if constexpr (M == 32) return (uint32_t)__shfl_xor((int)v, 32, kWave);
+    else return (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, M << 10 | 0x1f);
+}
+// Bit l: whether element BASE + l keeps the larger of the two that meet in this step of a bitonic network for descending order.
+constexpr uint64_t keeps_larger(int base, int size, int stride) {
+    uint64_t m = 0;
+    for (int l = 0; l < 64; l++)
+        if ((((base + l) & stride) == 0) == (((base + l) & size) == 0)) m |= (uint64_t)1 << l;
+    return m;
+}
+template <int KEYS, int SIZE, int STRIDE>
+__device__ __forceinline__ void sort_step(uint64_t (&key)[KEYS]) {
+    if constexpr (STRIDE >= kWave) {  // (of two keys a lane, the last merge)
+        const uint64_t a = key[0], b = key[1];
+        key[0] = a > b ? a : b;
+        key[1] = a > b ? b : a;
+    } else {
+        auto step = [&](auto e_tag) {
+            constexpr int e = decltype(e_tag)::value;
+            constexpr uint64_t larger_mask = keeps_larger(e * kWave, SIZE, STRIDE);
+            const uint64_t other = (uint64_t)lane_xor<STRIDE>((uint32_t)(key[e] >> 32)) << 32 | lane_xor<STRIDE>((uint32_t)key[e]);
+            const bool keep = __builtin_amdgcn_inverse_ballot_w64(__ballot(key[e] > other) ^ ~larger_mask);
+            key[e] = keep ? key[e] : other;
+        };
+        step(std::integral_constant<int, 0>{});
+        if constexpr (KEYS == 2) step(std::integral_constant<int, 1>{});
+    }
+    if constexpr (STRIDE > 1) sort_step<KEYS, SIZE, STRIDE / 2>(key);
+    else if constexpr (SIZE < KEYS * kWave) sort_step<KEYS, SIZE * 2, SIZE>(key);
+}
+// A wave's candidates sorted in registers, KEYS of them a lane (of 64 keys 21 steps of six instructions; a rank costs four instructions
+// and a read of LDS for every two keys).
+template <int KEYS, int SEG, class Emit>
+__device__ __forceinline__ void emit_sorted(const Select<kWave, SEG>& s, const Place& at, uint32_t k, Emit emit) {
+    uint64_t key[KEYS];
+#pragma unroll
+    for (int e = 0; e < KEYS; e++) {
+        const uint32_t i = at.lane + e * kWave;
+        key[e] = i < at.n ? s.key[0][i] : 0;
+    }
+    sort_step<KEYS, 2, 1>(key);
+#pragma unroll
+    for (int e = 0; e < KEYS; e++)
+        if ((uint32_t)(at.lane + e * kWave) < k) emit((uint32_t)(at.lane + e * kWave), key[e]);
+}
+
+// The k largest candidates in order: emit(rank, key).
+// SORT: for k beyond 16 (the sort's registers slow the rest down: 8 of 600 in 60000 rows 42 us with it in the kernel, 37 without; 64 of
+// 1000 in 16384 rows 29 with it, 33 by ranks).
+template <int NT, bool SORT, int SEG, class Emit>
+__device__ __forceinline__ void select_emit(Select<NT, SEG>& s, Place& at, uint32_t k, Emit emit) {
     constexpr int kWaves = Select<NT>::kWaves;
     uint32_t all = 0;
     auto total = [&]() {
@@ -425,12 +484,16 @@ __device__ __forceinline__ void select_emit(Select<NT>& s, Place& at, uint32_t k
         }
     };
     total();
-    if (all > k + k / 2 + 16) {
+    if (SORT && NT == kWave ? all > 2 * kWave : all > k + k / 2 + 16) {
         constexpr int kKeys = NT == kWave ? kThin : 2;
         if (select_most<NT>(s, at) <= kKeys * kWave) {
             select_thin<NT, kKeys>(s, at, (k + kWaves - 1) / kWaves);
             total();
         }
+    }
+    if constexpr (NT == kWave && SORT) {
+        if (all <= kWave) return emit_sorted<1>(s, at, k, emit);
+        if (all <= 2 * kWave) return emit_sorted<2>(s, at, k, emit);
     }
     if (all > kRankMost && all > k) {
         select_cut<NT>(s, at, k);
@@ -460,15 +523,15 @@ __device__ __forceinline__ void select_emit(Select<NT>& s, Place& at, uint32_t k
     }
 }
 
-template <int NT, int VPT, int U, bool BEYOND>
-__global__ __launch_bounds__(256, U > 4 ? 3 : 4) void topk_kernel(const float* x, float* values, uint64_t* indices, size_t rows, uint32_t cols,
+template <int NT, int VPT, int U, bool BEYOND, bool SORT, int SEG, int PER_CU>
+__global__ __launch_bounds__(256, PER_CU) void topk_kernel(const float* x, float* values, uint64_t* indices, size_t rows, uint32_t cols,
                                                       uint32_t k) {
     constexpr int kRows = 256 / NT;
-    __shared__ Select<NT> mem[kRows];
+    __shared__ Select<NT, SEG> mem[kRows];
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));  // scalars: the row and its pieces' base are then too
     Place at{(int)(threadIdx.x % NT), NT == kWave ? 0 : w, (int)(threadIdx.x % kWave), 0u, 0u};
     const int sub = NT == kWave ? w : 0;
-    Select<NT>& s = mem[sub];
+    Select<NT, SEG>& s = mem[sub];
     const size_t step = (size_t)gridDim.x * kRows;
     size_t r = (size_t)blockIdx.x * kRows + sub;
     if (r >= rows) return;  // (only waves that own a row of their own: no barrier is missed)
@@ -477,7 +540,7 @@ __global__ __launch_bounds__(256, U > 4 ? 3 : 4) void topk_kernel(const float* x
     for (; r < rows; r += step) {
         const float* row = x + r * cols;
         select_row<NT, VPT, U, BEYOND>(s, at, v, row, r + step < rows ? x + (r + step) * cols : nullptr, cols, k);
-        select_emit<NT>(s, at, k, [&](uint32_t rank, uint64_t key) {
+        select_emit<NT, SORT>(s, at, k, [&](uint32_t rank, uint64_t key) {
             const uint32_t c = ~(uint32_t)key;
             float v = key_value((uint32_t)(key >> 32));
             if (v == 0.f || v != v) v = row[c];  // the key knows neither the sign of a zero nor which NaN it was
@@ -500,7 +563,7 @@ __global__ __launch_bounds__(256, 4) void topk_segments_kernel(const float* x, u
     float4u v[4];
     load_tile<256, 4, false>(v, at, part, n);
     select_row<256, 4, 4, false>(s, at, v, part, nullptr, n, k);
-    select_emit<256>(s, at, k, [&](uint32_t rank, uint64_t key) {
+    select_emit<256, true>(s, at, k, [&](uint32_t rank, uint64_t key) {
         keys[((size_t)blockIdx.x) * k + rank] = (key & ~(uint64_t)0xffffffffu) | (uint32_t)~(~(uint32_t)key + c0);
     });
 }
@@ -536,7 +599,7 @@ __global__ __launch_bounds__(256, 4) void topk_join_kernel(const float* x, const
         at.keyed = at.n;
         if (i0 % (256 * 8) == 0) __syncthreads();
     }
-    select_emit<256>(s, at, k, [&](uint32_t rank, uint64_t key) {
+    select_emit<256, true>(s, at, k, [&](uint32_t rank, uint64_t key) {
         const uint32_t c = ~(uint32_t)key;
         float v = key_value((uint32_t)(key >> 32));
         if (v == 0.f || v != v) v = x[r * cols + c];
@@ -1505,12 +1568,18 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
                "topk_fwd: an output overlaps another operand");
     DeviceGuard guard(ctx);
     const uint32_t c32 = (uint32_t)cols, k32 = (uint32_t)k;
-#define ZG_TOPK(NT, VPT, U, BEYOND)                                                                                      \
-    hipLaunchKernelGGL((topk_kernel<NT, VPT, U, BEYOND>), dim3(grid(256 / (NT), U)), dim3(256), 0, ctx->stream, x, values,       \
-                       indices, rows, c32, k32)
+#define ZG_TOPK_(NT, VPT, U, BEYOND, SORT, SEG, PER_CU)                                                                                \
+    hipLaunchKernelGGL((topk_kernel<NT, VPT, U, BEYOND, SORT, SEG, PER_CU>), dim3(grid(256 / (NT), PER_CU)), dim3(256), 0, ctx->stream, \
+                       x, values, indices, rows, c32, k32)
+#define ZG_TOPK_WAVE(VPT, SEG, PER_CU)                                \
+    do {                                                              \
+        if (k > 16) ZG_TOPK_(64, VPT, 4, false, true, SEG, PER_CU);   \
+        else ZG_TOPK_(64, VPT, 4, false, false, SEG, PER_CU);         \
+    } while (0)
+#define ZG_TOPK(NT, VPT, U, BEYOND) ZG_TOPK_(NT, VPT, U, BEYOND, true, kSegment, (U > 4 ? 3 : 4))
     // as many workgroups as the compute units hold, with the same number of rows each
-    auto grid = [&](size_t per_block, int u) {
-        const size_t blocks = ceil_div_sz(rows, per_block), most = (size_t)ctx->n_cu * (u > 4 ? 3 : 4);
+    auto grid = [&](size_t per_block, size_t per_cu) {
+        const size_t blocks = ceil_div_sz(rows, per_block), most = ctx->n_cu * per_cu;
         return (unsigned)ceil_div_sz(blocks, ceil_div_sz(blocks, most));
     };
     // A few long rows are cut into segments, which takes two launches (64 of 128000: 1 row 16 us against 39 us with a workgroup per
@@ -1542,10 +1611,10 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
         else if (cols <= 128) ZG_TOPK_SHORT(16, 8);
         else ZG_TOPK_SHORT(16, 16);
     } else if (k <= 128 && (cols <= 2048 || rows >= (size_t)ctx->n_cu * 8)) {
-        if (cols <= 256) ZG_TOPK(64, 1, 4, false);
-        else if (cols <= 512) ZG_TOPK(64, 2, 4, false);
-        else if (cols <= 1024) ZG_TOPK(64, 4, 4, false);
-        else if (cols <= 2048) ZG_TOPK(64, 8, 4, false);
+        if (cols <= 256) ZG_TOPK_WAVE(1, 256, 8);
+        else if (cols <= 512) ZG_TOPK_WAVE(2, 512, 7);
+        else if (cols <= 1024) ZG_TOPK_WAVE(4, 512, 6);
+        else if (cols <= 2048) ZG_TOPK_WAVE(8, 512, 4);
         else if (cols <= 8192) ZG_TOPK(64, 8, 4, true);
         else ZG_TOPK(64, 4, 6, true);  // fewer waves with more on its way each (64 of 32000 in 8192 rows: 182 us against 202)
     } else if (cols <= 2048) {
@@ -1559,6 +1628,8 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
     }
 #undef ZG_TOPK_SHORT
 #undef ZG_TOPK
+#undef ZG_TOPK_WAVE
+#undef ZG_TOPK_
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
 }
