@@ -99,7 +99,8 @@ int zg_hip_expert_combine_bwd(zg_hip_ctx *ctx, const float *out_g, const float *
  *   forward   y = x w_e^T + bias_e (null: none), max(0, .) when relu
  *   backward  gw_e += gy_e^T x_e;  gb_e += column sums of gy_e (null: none);  gx = gy w_e, zero where act_in <= 0 (gx null: no
  *             input gradient, w is not read; act_in null: no mask).  accumulate == 0: gw and gb are written, zero for an
- *             expert without rows.  A layer without inputs or outputs: nothing to do.  Uses the workspace when there are more than 64 experts or gb is given.
+ *             expert without rows.  A layer without inputs or outputs: nothing to do.  Uses the workspace when there
+ *             are more than 64 experts, when gb is given, and for layers so small that the rows are cut into parts.
  * ------------------------------------------------------------------------------------------- */
 int zg_hip_expert_linear_fwd(zg_hip_ctx *ctx, const float *x, const float *w, const float *bias, float *y,
                              const uint64_t *offsets, size_t n_rows, size_t n_experts, size_t fan_in, size_t fan_out, int relu);

@@ -151,6 +151,24 @@ def test_many_experts_of_many_rows(hip, n_experts, per, fan_in, fan_out):
     check_bwd(hip, c, False, False, False, shift=1)
 
 
+@pytest.mark.parametrize("counts,behind,fan_in,fan_out", [([515], 0, 20, 30), ([4000], 3, 64, 130), ([3000, 0, 1], 5, 96, 63), ([0, 2500, 900], 0, 17, 70),
+                                                          ([34000] + [1, 0, 5] * 21 + [40], 2, 20, 12), ([129] * 3 + [2000], 0, 260, 65)])
+def test_small_layers_with_many_rows(hip, counts, behind, fan_in, fan_out):
+    """The rows of an expert in parts for its weight gradient, added up afterwards; parts without a row."""
+    c = case(len(counts) + fan_in, counts, behind, fan_in, fan_out)
+    check_fwd(hip, c, True, True)
+    for bias, mask, accumulate in ((True, True, True), (False, False, False)):
+        check_bwd(hip, c, bias, mask, accumulate, shift=1 if accumulate else 0)
+
+
+@pytest.mark.parametrize("rows", [1, 17, 40, 100, 250, 1030])
+@pytest.mark.parametrize("fan_in,fan_out", [(100, 260), (1030, 64), (64, 1000)])
+def test_one_expert(hip, rows, fan_in, fan_out):
+    c = case(rows, [rows], 1, fan_in, fan_out)
+    check_fwd(hip, c, True, True)
+    check_bwd(hip, c, True, True, True)
+
+
 @pytest.mark.parametrize("n,e,fan_in,fan_out", [(4500, 70, 68, 1920), (10500, 5, 302, 1660), (2700, 3, 200, 6143)])
 def test_wide_tiles(hip, n, e, fan_in, fan_out):
     """Enough tiles of 64 x 128 for all compute units, forward or in the input gradient, the last column of tiles whole or not."""

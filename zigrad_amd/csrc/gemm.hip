@@ -396,6 +396,13 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_kernel(GemmArgs g) {
         z = (size_t)(unsigned)__builtin_amdgcn_readfirstlane((int)z);
         first = (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
         count = (uint32_t)__builtin_amdgcn_readfirstlane((int)count);
+        if (gridDim.y > 1) {  // one part of the expert's rows, whose product goes to a buffer of its own
+            const uint32_t lo = (uint32_t)((uint64_t)count * blockIdx.y / gridDim.y), hi = (uint32_t)((uint64_t)count * (blockIdx.y + 1) / gridDim.y);
+            first += lo;
+            count = hi - lo;
+            g.C += blockIdx.y * g.split_stride;
+            split = 0;
+        }
         tile_coords(xcd_contiguous(blockIdx.x, g.tiles_m * g.tiles_n), g.tiles_m, g.tiles_n, tm, tn);
         g.K = count;
         g.A += (size_t)first * g.lda;
@@ -2749,18 +2756,21 @@ static int expert_rows(zg_hip_ctx* ctx, const float* A, const float* B, float* C
     g.c_vec = aligned16(C) && n % 4 == 0 && (!gate || aligned16(gate));
     g.bounded_tail = !B_KMAJOR && n % 4 != 0;
     // Few rows per expert: the kernel above, with 16 x 16 or 32 x 32 blocks, as long as it reads the weights once or twice only or the
-    // staged kernel's 64 x 64 tiles do not fill the compute units (measured at 8 to 64 experts of 300 x 500 to 4096 x 4096).
+    // staged kernel's 64 x 64 tiles do not fill the compute units (measured at 1 to 64 experts of 300 x 500 to 4096 x 4096).
     // k-contiguous weights (forward), 1024 -> 2048, 8 experts: 32 rows 11 against 21 us, 256 rows 29 against 35, 512 rows 39
     // against 36; 1024 -> 1024, 64 experts: 1024 rows 56 against 64, 2048 rows 84 against 65.
     // Weights read value by value (input gradient), the same layers: 32 rows 17 against 42 us, 256 rows 31 against 43; 64 experts:
     // 64 rows 33 against 44, 256 rows 59 against 51.
+    // With so few tiles that three compute units of four would have none the small blocks win at any number of rows, though they read
+    // the weights many times (one expert, forward: 1024 -> 1024, 48 rows 6.7 against 10.7 us, 200 rows 16.5 against 19.9; 512 -> 512, 400
+    // rows 10.2 against 12.3; 1024 -> 64, 4000 rows 18.2 against 19.8; 200 rows 1024 -> 2048, half of the compute units: 27 against 20).
     const size_t per = n_rows / n_experts, n_cu = (size_t)ctx->n_cu;
     const size_t tiles = (n_rows / 64 + (n_rows < n_experts ? n_rows : n_experts)) * ceil_div_sz(n, 64);
     if (B_KMAJOR) {
-        if (per <= 6) return launch_expert_few<1, 1, 8, B_KMAJOR>(ctx, g);
+        if (per <= 6 || tiles <= n_cu / 4 || (per <= 16 && tiles <= n_cu)) return launch_expert_few<1, 1, 8, B_KMAJOR>(ctx, g);
         if (per <= 20 || (per <= 48 && tiles <= n_cu)) return launch_expert_few<2, 2, 4, B_KMAJOR>(ctx, g);
     } else {
-        if (per <= 2 || (per <= 16 && tiles <= n_cu)) return launch_expert_few<1, 1, 8, B_KMAJOR>(ctx, g);
+        if (per <= 2 || tiles <= n_cu / 4 || (per <= 16 && tiles <= n_cu)) return launch_expert_few<1, 1, 8, B_KMAJOR>(ctx, g);
         if (per <= 32 && tiles <= 3 * n_cu) return launch_expert_few<2, 2, 4, B_KMAJOR>(ctx, g);
     }
     // 64 x 128 tiles where eight a compute unit average out and the last column of tiles is as full as with 64 x 64 (1024 -> 2048, 16
@@ -2771,14 +2781,14 @@ static int expert_rows(zg_hip_ctx* ctx, const float* A, const float* B, float* C
     if (wide >= 8 * n_cu && ceil_div_sz(n, 64) % 2 == 0) return launch_expert_rows<64, 128, B_KMAJOR>(ctx, g);
     return launch_expert_rows<64, 64, B_KMAJOR>(ctx, g);
 }
-// C_e (+)= A[rows of e]^T B[rows of e]
+// C_e (+)= A[rows of e]^T B[rows of e], or the products of `parts` parts of an expert's rows, g.split_stride apart
 template <int BM, int BN>
-static int launch_expert_weights(zg_hip_ctx* ctx, GemmArgs g) {
+static int launch_expert_weights(zg_hip_ctx* ctx, GemmArgs g, unsigned parts) {
     g.tiles_m = (unsigned)ceil_div_sz(g.M, BM);
     g.tiles_n = (unsigned)ceil_div_sz(g.N, BN);
     ZG_REQUIRE((size_t)g.tiles_m * g.tiles_n < 0x7fffffffull, "expert_linear_bwd: a layer of %zu x %zu", g.M, g.N);
     constexpr size_t lds = 2 * (size_t)(Tile<BM, false>::ELEMS + Tile<BN, false>::ELEMS) * sizeof(float);
-    hipLaunchKernelGGL((gemm_kernel<BM, BN, false, false, 1, false, 2>), dim3(g.tiles_m * g.tiles_n, 1, g.n_experts),
+    hipLaunchKernelGGL((gemm_kernel<BM, BN, false, false, 1, false, 2>), dim3(g.tiles_m * g.tiles_n, parts, g.n_experts),
                        dim3(kGemmThreads), lds, ctx->stream, g);
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
@@ -2884,7 +2894,7 @@ __global__ __launch_bounds__(1024) void expert_order_kernel(const uint64_t* offs
 
 // Column sums of the experts' rows: 32 lanes of four columns by 8 row-threads with eight rows in flight.  Each expert's rows are cut
 // into gridDim.z parts, so that one expert with most of the rows does not hold up the rest; a part's sums go to `out` (laid out
-// [part][expert][column]), which expert_bias_join_kernel adds up in order, or, with a single part, to the gradient itself.
+// [part][expert][column]), which expert_join_kernel adds up in order, or, with a single part, to the gradient itself.
 template <bool ACC>
 __global__ __launch_bounds__(256) void expert_bias_grad_kernel(const float* gy, float* out, const uint64_t* offsets, size_t n_rows,
                                                                 size_t fan_out) {
@@ -2932,12 +2942,13 @@ __global__ __launch_bounds__(256) void expert_bias_grad_kernel(const float* gy, 
         to[e] = ACC ? to[e] + s : s;
     }
 }
-__global__ __launch_bounds__(256) void expert_bias_join_kernel(const float* parts, float* gb, size_t n, unsigned n_parts, int accumulate) {
+// The parts of n sums, in order.
+__global__ __launch_bounds__(256) void expert_join_kernel(const float* parts, float* to, size_t n, unsigned n_parts, int accumulate) {
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     float s = 0.f;
     for (unsigned p = 0; p < n_parts; p++) s += parts[(size_t)p * n + i];
-    gb[i] = accumulate ? gb[i] + s : s;
+    to[i] = accumulate ? to[i] + s : s;
 }
 }  // namespace zg
 
@@ -2987,13 +2998,24 @@ ZG_API int zg_hip_expert_linear_bwd(zg_hip_ctx* ctx, const float* gy, const floa
     g.bounded_tail = fan_out % 4 != 0 || fan_in % 4 != 0;
     // few rows: the kernel that writes wide (64 experts of 512 x 512, 512 rows: 28 against 32 us, 1024 rows: 44 against 34)
     const bool few = n_rows / n_experts <= 8;
-    // workspace: the experts' order, then the parts of the bias gradient
+    // 128 x 128 tiles where there are several for every compute unit (16 experts of 2048 x 1024, 16384 rows: 490 us against 548 with
+    // 64 x 64), else the smaller ones (64 experts of 512 x 512, 4096 rows, one expert with 609: 88 us the three products against 96)
+    const bool large = n_experts * ceil_div_sz(fan_out, 128) * ceil_div_sz(fan_in, 128) >= 6 * (size_t)ctx->n_cu;
+    // An expert's rows in four parts or more, of 128 or more, where the tiles alone leave compute units without one (the whole backward of
+    // 1024 -> 64 for 4000 rows of one expert: 46 us against 110, of 64 -> 64 for 16384 rows of four: 45 against 198).  Two or three parts
+    // do not pay for the launch that adds them up (256 -> 256, 300 rows: 22 us against 21).
+    const size_t tiles = n_experts * ceil_div_sz(fan_out, 64) * ceil_div_sz(fan_in, 64), n_weights = n_experts * fan_out * fan_in;
+    size_t w_parts = few || tiles >= (size_t)ctx->n_cu ? 1 : 2 * (size_t)ctx->n_cu / tiles;
+    if (w_parts > n_rows / (n_experts * 128)) w_parts = n_rows / (n_experts * 128);
+    if (w_parts < 4) w_parts = 1;
+    // workspace: the experts' order, the parts of the weight gradient, those of the bias gradient
     const size_t order_bytes = n_experts > kWave && !few ? (n_experts * sizeof(uint32_t) + 255) / 256 * 256 : 0;
     size_t parts = 1;  // about 128 rows of an average expert each
     if (gb) parts = n_rows / (n_experts * 128);
-    if (parts > 16) parts = 16;
+    if (parts > 64) parts = 64;
     if (parts < 1) parts = 1;
-    const size_t need = order_bytes + (gb && parts > 1 ? parts * n_experts * fan_out * sizeof(float) : 0);
+    const size_t w_bytes = w_parts > 1 ? (w_parts * n_weights * sizeof(float) + 255) / 256 * 256 : 0;
+    const size_t need = order_bytes + w_bytes + (gb && parts > 1 ? parts * n_experts * fan_out * sizeof(float) : 0);
     char* ws = nullptr;
     if (need) {
         ws = (char*)workspace(ctx, need);
@@ -3014,14 +3036,23 @@ ZG_API int zg_hip_expert_linear_bwd(zg_hip_ctx* ctx, const float* gy, const floa
             ZG_LAUNCH_CHECK();
             g.order = (const uint32_t*)ws;
         }
-        // 128 x 128 tiles where there are several for every compute unit (16 experts of 2048 x 1024, 16384 rows: 490 us against 548 with
-        // 64 x 64), else the smaller ones (64 experts of 512 x 512, 4096 rows, one expert with 609: 88 us the three products against 96)
-        const bool large = n_experts * ceil_div_sz(fan_out, 128) * ceil_div_sz(fan_in, 128) >= 6 * (size_t)ctx->n_cu;
-        if (int rc = large ? launch_expert_weights<128, 128>(ctx, g) : launch_expert_weights<64, 64>(ctx, g)) return rc;
+        if (w_parts > 1) {
+            g.C = (float*)(ws + order_bytes);
+            g.c_vec = fan_in % 4 == 0;
+            g.beta = 0.f;
+            g.split_stride = n_weights;
+        }
+        if (int rc = large ? launch_expert_weights<128, 128>(ctx, g, (unsigned)w_parts) : launch_expert_weights<64, 64>(ctx, g, (unsigned)w_parts))
+            return rc;
+        if (w_parts > 1) {
+            hipLaunchKernelGGL(expert_join_kernel, dim3((unsigned)ceil_div_sz(n_weights, 256)), dim3(256), 0, ctx->stream, g.C, gw, n_weights,
+                               (unsigned)w_parts, accumulate ? 1 : 0);
+            ZG_LAUNCH_CHECK();
+        }
     }
     if (gb) {
         const dim3 grid((unsigned)ceil_div_sz(fan_out, 128), (unsigned)n_experts, (unsigned)parts);
-        float* out = parts > 1 ? (float*)(ws + order_bytes) : gb;
+        float* out = parts > 1 ? (float*)(ws + order_bytes + w_bytes) : gb;
         if (parts == 1 && accumulate)
             hipLaunchKernelGGL(expert_bias_grad_kernel<true>, grid, dim3(256), 0, ctx->stream, gy, out, offsets, n_rows, fan_out);
         else
@@ -3029,7 +3060,7 @@ ZG_API int zg_hip_expert_linear_bwd(zg_hip_ctx* ctx, const float* gy, const floa
         ZG_LAUNCH_CHECK();
         if (parts > 1) {
             const size_t n = n_experts * fan_out;
-            hipLaunchKernelGGL(expert_bias_join_kernel, dim3((unsigned)ceil_div_sz(n, 256)), dim3(256), 0, ctx->stream, out, gb, n,
+            hipLaunchKernelGGL(expert_join_kernel, dim3((unsigned)ceil_div_sz(n, 256)), dim3(256), 0, ctx->stream, out, gb, n,
                                (unsigned)parts, accumulate ? 1 : 0);
             ZG_LAUNCH_CHECK();
         }
