@@ -737,52 +737,54 @@ __device__ __forceinline__ void add_entries(float* at, float g, uint64_t same, i
     if (writes) *at = v;
 }
 
-// The same for any row: NT threads (a wave up to 1024 columns, else a workgroup) put together 16 NT columns in LDS, which holds zeros
-// but for the entries that one wave adds, 64 at a time, and that are taken out again once the span is stored.  (Clearing the span in
-// memory and writing the entries after it, each a part of a line, took 241 us for 64 of 32000 in 8192 rows, this 184 us, 5.7 TB/s;
-// stores past the cache 205, and 23 against 16 us for 583 rows of 41270.  65536 rows of 300 by workgroups: 54 us, by waves 23.)
+// The same for any row: NT threads (a wave up to 1024 columns, else a workgroup for each of even spans) put together up to 16 NT columns in
+// LDS: zeros, then the entries, which one wave adds 64 at a time, then whole pieces to memory.  (64 of 32000 in 8192 rows: 202 us, 5.2
+// TB/s; clearing the span in memory and writing the entries after it, each a part of a line, 241.  Stores past the cache take 23
+// us for 583 rows of 41270, these 15.  65536 rows of 300 by workgroups: 54 us, by waves 19.)
 __device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 template <int NT>
 __global__ __launch_bounds__(256) void topk_bwd_kernel(const uint64_t* indices, const float* y_g, float* x_g, size_t rows,
-                                                       uint32_t cols, uint32_t k, uint32_t spans, int bits) {
+                                                       uint32_t cols, uint32_t k, uint32_t spans, uint32_t span_cols, int bits) {
     constexpr uint32_t kSpan = 16 * NT;
     __shared__ __attribute__((aligned(16))) float span_mem[256 / NT * kSpan];
     const int lane = threadIdx.x % kWave, tid = threadIdx.x % NT;
     const int sub = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / NT));
     float* const span = span_mem + sub * kSpan;
-    const bool first = tid < kWave;
-    for (uint32_t c = tid; c < kSpan; c += NT) span[c] = 0.f;
-    const size_t jobs = rows * spans;
-    for (size_t job = (size_t)blockIdx.x * (256 / NT) + sub; job < jobs; job += (size_t)gridDim.x * (256 / NT)) {
-        const size_t r = job / spans;
-        const uint32_t c0 = (uint32_t)(job - r * spans) * kSpan, n = cols - c0 < kSpan ? cols - c0 : kSpan;
-        float* row = x_g + r * cols + c0;
-        select_sync<NT>();
-        if (first) {
-            for (uint32_t j0 = 0; j0 < k; j0 += kWave) {
-                const uint64_t at = (j0 + lane < k ? indices[r * k + j0 + lane] : ~(uint64_t)0) - c0;
-                const bool here = at < n;
-                const uint64_t heres = __ballot(here);
-                if (!heres) continue;
+    const size_t job = (size_t)blockIdx.x * (256 / NT) + sub, r = job / spans;
+    if (r >= rows) return;  // (only waves with rows of their own: no barrier is missed)
+    const uint32_t c0 = (uint32_t)(job - r * spans) * span_cols, n = cols - c0 < span_cols ? cols - c0 : span_cols;
+    float* row = x_g + r * cols + c0;
+    uint64_t idx = ~(uint64_t)0;
+    float g = 0.f;
+    if (tid < kWave && (uint32_t)lane < k) {
+        idx = indices[r * k + lane];
+        g = y_g[r * k + lane];
+    }
+    for (uint32_t c = 4 * tid; c < n; c += 4 * NT) *reinterpret_cast<float4*>(span + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+    select_sync<NT>();
+    if (tid < kWave) {
+        for (uint32_t j0 = 0;;) {
+            const uint64_t at = idx - c0;
+            const bool here = at < n;
+            const uint64_t heres = __ballot(here);
+            if (heres) {
                 const uint32_t col = here ? (uint32_t)at : 0u;
-                const float g = here ? y_g[r * k + j0 + lane] : 0.f;
                 uint64_t same = same_lanes(col, bits, heres);
                 if (!here) same = 0;
-                add_entries<false>(span + col, g, same, lane);
+                add_entries<false>(span + col, here ? g : 0.f, same, lane);
                 select_sync<kWave>();
             }
+            j0 += kWave;
+            if (j0 >= k) break;
+            const bool live = j0 + lane < k;
+            idx = live ? indices[r * k + j0 + lane] : ~(uint64_t)0;
+            g = live ? y_g[r * k + j0 + lane] : 0.f;
         }
-        select_sync<NT>();
-        uint32_t c = 4 * tid;
-        for (; c + 4 <= n; c += 4 * NT) *reinterpret_cast<float4u*>(row + c) = *reinterpret_cast<const float4u*>(span + c);
-        for (; c < n; c++) row[c] = span[c];
-        select_sync<NT>();
-        if (first)
-            for (uint32_t j = lane; j < k; j += kWave) {
-                const uint64_t at = indices[r * k + j] - c0;
-                if (at < n) span[at] = 0.f;
-            }
     }
+    select_sync<NT>();
+    uint32_t c = 4 * tid;
+    for (; c + 4 <= n; c += 4 * NT) *reinterpret_cast<float4u*>(row + c) = *reinterpret_cast<const float4u*>(span + c);
+    for (; c < n; c++) row[c] = span[c];
 }
 // Adding to what is there: a wave takes as many rows as it has lanes for, or one of more than 64 places.
 __global__ __launch_bounds__(256) void topk_bwd_add_kernel(const uint64_t* indices, const float* y_g, float* x_g, size_t rows,
@@ -1659,20 +1661,16 @@ ZG_API int zg_hip_topk_bwd(zg_hip_ctx* ctx, const uint64_t* indices, const float
         else if (cols <= 128) hipLaunchKernelGGL(topk_bwd_short_kernel<2>, grid, dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32);
         else hipLaunchKernelGGL(topk_bwd_short_kernel<4>, grid, dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32);
     } else {
-        // one span after another, four at most, once there are enough for all compute units (the start of a workgroup clears a span of its own: 215 rows of 1310
-        // one each 4.4 us, four each 7.1; 8192 rows of 1000 one each 13.3, four each 11.3)
-        auto grid = [&](size_t blocks) {
-            const size_t all = 8 * (size_t)ctx->n_cu;
-            return dim3(row_grid(blocks <= all ? blocks : blocks < 4 * all ? all : ceil_div_sz(blocks, 4)));
-        };
-        if (cols <= 1024) {
-            hipLaunchKernelGGL(topk_bwd_kernel<64>, grid(ceil_div_sz(rows, 4)), dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32,
-                               k32, 1u, bits);
-        } else {
-            const uint32_t spans = (uint32_t)ceil_div_sz(cols, 4096);
-            hipLaunchKernelGGL(topk_bwd_kernel<256>, grid(rows * spans), dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32,
-                               spans, bits < 12 ? bits : 12);
-        }
+        // even spans of whole 128-byte lines
+        const size_t span = cols <= 1024 ? cols : (ceil_div_sz(cols, ceil_div_sz(cols, 4096)) + 31) / 32 * 32;
+        const size_t spans = ceil_div_sz(cols, span), blocks = cols <= 1024 ? ceil_div_sz(rows, 4) : mul_sat(rows, spans);
+        ZG_REQUIRE(blocks < 0x7fffffffull, "topk_bwd: %zu rows of %zu columns", rows, cols);
+        if (cols <= 1024)
+            hipLaunchKernelGGL(topk_bwd_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32,
+                               (uint32_t)spans, (uint32_t)span, bits);
+        else
+            hipLaunchKernelGGL(topk_bwd_kernel<256>, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32,
+                               (uint32_t)spans, (uint32_t)span, bits < 12 ? bits : 12);
     }
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
