@@ -4,7 +4,7 @@ It mirrors the device interface Zigrad's upper layers program against
 (reference: src/device/device_reference.zig:15-131): `dispatch(name, **params)` takes the op name and
 the field names of the matching parameter struct in src/device/opspec.zig, and the `mem_*` methods
 keep the names and meaning of the reference's memory API.  Every call goes through the C ABI in
-include/zg_hip.h; nothing is computed in Python and nothing falls back to the CPU.
+include/zg_hip.h and include/zg_hip_topk.h; nothing is computed in Python and nothing falls back to the CPU.
 
 Slices of the reference (`[]T`) are `DevBuf` objects here: a device pointer, an element count and a
 dtype.  `DevBuf.sub(offset, n)` is the pointer-arithmetic sub-slice the reference takes freely
