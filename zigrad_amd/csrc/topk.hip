@@ -609,8 +609,9 @@ __global__ __launch_bounds__(256, 4) void topk_join_kernel(const float* x, const
 }
 
 // Short rows and few of their values chosen (a router's scores): L lanes share a row, each holding KPL adjacent columns as keys in
-// registers, and the largest is taken out k times (8 of 128 in 65536 rows: 15 us, a wave per row with a bound and candidates 45 us).  A round is a handful of maxima across the lanes; a tie goes to the lowest lane
-// and there to the lowest column, which is the lowest column of the row.
+// registers, and the largest is taken out k times (8 of 128 in 65536 rows: 15 us, a wave per row with a bound and candidates 29 us).
+// A round is a handful of maxima across the lanes; a tie goes to the lowest lane and there to the lowest column, which is the lowest
+// column of the row.
 template <int L>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
     auto step = [&](auto ctrl) {
@@ -813,10 +814,12 @@ __global__ __launch_bounds__(256) void topk_bwd_add_kernel(const uint64_t* indic
 // Distillation.  With c = log2(e) / T and m, tm the largest logit of the student and the teacher:
 //   e_c = 2^((x_c - m) c), s = sum e_c, p_c = e_c / s      f_j = 2^((t_j - tm) c), S = sum f_j, q_j = f_j / S
 //   row_loss = T^2 (sum_j f_j ((t_j - tm) - (x_{i_j} - m)) / T / S - log S + log s)
-// A row's logits are read once, into registers, by 16 lanes, a wave, or a workgroup of 256 or 1024, by its length (rows of
-// more than 65536 columns are read twice for the gradient); the maxima, then all sums, take one reduction each.  For the gradient the q_j go into a
-// stretch of LDS laid out like the row, from where every thread takes what belongs to its columns: the gradient leaves in whole
-// 16-byte pieces, written once, and a class that is named twice gets both shares, added in the order of j by one wave.
+// A row's logits are read once, into registers, by 16 lanes, a wave, or a workgroup of 256, 512 or 1024, by its length (the loss alone
+// reads rows of more than 32768 columns with a running maximum; for more than 65536 the gradient reads them again); the maxima, then
+// all sums, take one reduction each.  Bound by memory: 8192 x 32000 forward 155 us, 6.8 TB/s.  In the gradient of rows of up to 2048
+// columns the q_j go into a stretch of LDS laid out like the row, from where every thread takes what belongs to its columns; of longer
+// rows the few classes that have a share are written a second time.  Either way a class that is named twice gets both shares,
+// added in the order of j.
 // ------------------------------------------------------------------------------------------------
 struct DistillArgs {
     const float* x;
@@ -1607,7 +1610,8 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
 #define ZG_TOPK_SHORT(L, KPL)                                                                                                    \
     hipLaunchKernelGGL((topk_short_kernel<L, KPL>), dim3((unsigned)ceil_div_sz(rows, 256 / (L))), dim3(256), 0, ctx->stream, x,      \
                        values, indices, rows, c32, k32)
-    if (cols <= 256 && k <= 16) {
+    // (8 of 128 in 65536 rows 15 us against 29 by a wave per row, 4 of 200 25 against 26, 8 of 256 34 against 29, 16 of 256 48 against 30)
+    if (cols <= 256 && k <= (cols <= 128 ? 16u : 4u)) {
         if (cols <= 16) ZG_TOPK_SHORT(4, 4);
         else if (cols <= 64) ZG_TOPK_SHORT(16, 4);
         else if (cols <= 128) ZG_TOPK_SHORT(16, 8);
