@@ -69,7 +69,8 @@ int zg_hip_distill_fwd_bwd(zg_hip_ctx *ctx, const float *logits, const float *te
  * not below n_experts drops the entry (a full expert, a padding row).
  *   expert_sort      orders the entries by expert, those of one expert by i: slots[i] = the entry's place in that order,
  *                    UINT64_MAX for a dropped one; expert e owns the places offsets[e] .. offsets[e + 1] - 1.  offsets has
- *                    n_experts + 1 entries.  1 <= n_experts <= ZG_HIP_EXPERTS_MAX, n_entries < 2^32.  Uses the workspace.
+ *                    n_experts + 1 entries.  1 <= n_experts <= ZG_HIP_EXPERTS_MAX, n_entries < 2^32 - 1.  Uses the workspace
+ *                    beyond 2048 entries.
  *   expert_dispatch  y[slots[t * k + j], :] = x[t, :].  y has n_tokens * k rows; those behind the last place are left as they were.
  *   expert_dispatch_bwd  x_g[t, :] += sum over j of y_g[slots[t * k + j], :], in the order of j; accumulate == 0: written.
  *   expert_combine   out[t, :] = sum over j of weights[t, j] y[slots[t * k + j], :], in the order of j (zeros for a row with no

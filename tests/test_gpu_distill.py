@@ -93,6 +93,16 @@ def test_row_lengths_around_the_kernels_own(hip, cols, fused):
         check(run(hip, x, teacher, indices, 2.0, w, add, fused), x, teacher, indices, 2.0, w, add)
 
 
+@pytest.mark.parametrize("cols", [257, 511, 512, 513, 1024, 2048, 2049, 4096, 4097, 16384])
+@pytest.mark.parametrize("k", [64, 65, 257])
+@pytest.mark.parametrize("fused", [False, True])
+def test_numbers_of_entries(hip, cols, k, fused):
+    x, teacher, indices, grad0 = case(cols + k, 3, cols, k)
+    indices[1, 3:9] = indices[1, 2]  # one class seven times
+    for add in (None, grad0):
+        check(run(hip, x, teacher, indices, 1.5, None, add, fused), x, teacher, indices, 1.5, None, add)
+
+
 @pytest.mark.parametrize("cols", [10, 200, 5000, 33000, 70000])
 def test_extreme_temperatures(hip, cols):
     """At 1e-18 every row but those of equal logits has one class; at 1e18 all classes are equal and the loss is next to nothing."""

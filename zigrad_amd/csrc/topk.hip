@@ -1055,24 +1055,23 @@ __device__ __forceinline__ void span_shares(float* span, const uint32_t* col, co
 }
 
 // NT threads a row (a wave: four rows a workgroup), which they hold in VPT pieces of four columns each.  The gradient (of rows of a wave
-// only) takes its shares from a stretch of LDS.
-template <int NT, int VPT, bool FWD, bool BWD, bool ACC>
+// only) takes its shares from a stretch of LDS.  ENTRIES: the teacher's that a thread has, at most.
+template <int NT, int VPT, int ENTRIES, bool FWD, bool BWD, bool ACC>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 ? 8 : 1) void distill_row_kernel(DistillArgs a) {
     static_assert(!BWD || NT == kWave, "one wave fills the stretch and reads it");
     constexpr int kRows = NT < 256 ? 256 / NT : 1;
     constexpr uint32_t kSpan = 4 * NT * VPT;
-    constexpr int kBits = VPT == 4 ? 10 : 11;
+    constexpr int kBits = VPT == 2 ? 9 : VPT == 4 ? 10 : 11;
     static_assert(!BWD || kSpan == 1u << kBits, "bits of a column");
-    constexpr int kEntries = (kMaxK + NT - 1) / NT;
     __shared__ __attribute__((aligned(16))) float span_mem[BWD ? kRows * kSpan : 4];
-    __shared__ uint32_t col_mem[BWD ? kRows * kMaxK : 1];
-    __shared__ float q_mem[BWD ? kRows * kMaxK : 1];
+    __shared__ uint32_t col_mem[BWD ? kRows * ENTRIES * NT : 1];
+    __shared__ float q_mem[BWD ? kRows * ENTRIES * NT : 1];
     __shared__ float smem[NT > kWave ? 3 * (NT / kWave) : 1];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
     const int sub = NT == kWave ? wave : 0, tid = threadIdx.x % NT;
     float* const span = span_mem + (BWD ? sub * kSpan : 0);
-    uint32_t* const col_of = col_mem + (BWD ? sub * kMaxK : 0);
-    float* const q_of = q_mem + (BWD ? sub * kMaxK : 0);
+    uint32_t* const col_of = col_mem + (BWD ? sub * ENTRIES * NT : 0);
+    float* const q_of = q_mem + (BWD ? sub * ENTRIES * NT : 0);
     const size_t r = (size_t)blockIdx.x * kRows + sub;
     if (r >= a.rows) return;  // only waves that own a row of their own: no barrier is missed
     const uint32_t cols = a.cols, whole = cols & ~3u;
@@ -1093,11 +1092,11 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 ? 8 : 1) void disti
     float4u v[VPT];
     row_pieces<VPT>(v, x, bytes_from(0, whole), 16 * tid, 16 * NT, a.once);
     const float tail = whole + tid < cols ? x[whole + tid] : -INFINITY;  // of the first threads
-    uint32_t col[kEntries];
-    float t[kEntries], xe[kEntries];
+    uint32_t col[ENTRIES];
+    float t[ENTRIES], xe[ENTRIES];
     float top[2] = {-INFINITY, tail};
 #pragma unroll
-    for (int i = 0; i < kEntries; i++) {
+    for (int i = 0; i < ENTRIES; i++) {
         if (i == 0 || i * NT < (int)a.k) {
             teacher_entry(a, r, tid + i * NT, col[i], t[i]);
             xe[i] = FWD && col[i] != kNoCol ? x[col[i]] : 0.f;
@@ -1130,9 +1129,9 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 ? 8 : 1) void disti
     }
     const float from_x = m == -INFINITY ? 0.f : m, from_t = top[0] == -INFINITY ? 0.f : top[0];
     float sum[3] = {0.f, 0.f, 0.f};
-    float f[kEntries];
+    float f[ENTRIES];
 #pragma unroll
-    for (int i = 0; i < kEntries; i++) {
+    for (int i = 0; i < ENTRIES; i++) {
         float part;
         teacher_terms(a, t[i], xe[i], from_t, from_x, f[i], part);
         sum[0] += f[i];
@@ -1162,7 +1161,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, NT == 1024 ? 8 : 1) void disti
     if constexpr (BWD) {
         if (ACC && res.empty) return;
 #pragma unroll
-        for (int i = 0; i < kEntries; i++) {
+        for (int i = 0; i < ENTRIES; i++) {
             col_of[tid + i * NT] = col[i];
             q_of[tid + i * NT] = f[i] * res.inv_S;
         }
@@ -1475,21 +1474,31 @@ static int distill_launch(zg_hip_ctx* ctx, DistillArgs a, float* loss, bool* sum
         ZG_LAUNCH_CHECK();
         return ZG_HIP_OK;
     }
-#define ZG_ROWS(NT, VPT)                                                                                                        \
-    hipLaunchKernelGGL((distill_row_kernel<NT, VPT, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(a.rows, NT < 256 ? 256 / NT : 1)), \
+#define ZG_ROWS_(NT, VPT, ENTRIES)                                                                                                          \
+    hipLaunchKernelGGL((distill_row_kernel<NT, VPT, ENTRIES, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(a.rows, NT < 256 ? 256 / NT : 1)), \
                        dim3(NT < 256 ? 256 : NT), 0, ctx->stream, a)
+#define ZG_ROWS(NT, VPT)                                       \
+    do {                                                       \
+        if (a.k <= NT && few) ZG_ROWS_(NT, VPT, 1);            \
+        else ZG_ROWS_(NT, VPT, (kMaxK + NT - 1) / NT);         \
+    } while (0)
 #define ZG_GRAD(NT, R, L)                                                                                                              \
     do {                                                                                                                               \
         const dim3 grid((unsigned)(a.rows * a.segments));                                                                              \
         if (a.once) hipLaunchKernelGGL((distill_grad_kernel<NT, R, L, FWD, ACC, true>), grid, dim3(NT), 0, ctx->stream, a);            \
         else hipLaunchKernelGGL((distill_grad_kernel<NT, R, L, FWD, ACC, false>), grid, dim3(NT), 0, ctx->stream, a);                  \
     } while (0)
+    // One entry of the teacher a thread where that does (65536 rows of 600, k = 8: step 55 us against 78 with room for 512), but for the
+    // gradient that is added to in rows of more than 1024 columns (2000, k = 64: 300 us against 285).
+    const bool few = !ACC || a.cols <= 1024;
     // (the gradient alone: even segments)
     a.segments = FWD || a.cols <= 8192 ? 1u : (a.cols - 1) / 8192 + 1;
     a.segment = ((a.cols - 1) / a.segments + 4) & ~3u;
     a.segments = (a.cols - 1) / a.segment + 1;  // as many as have columns
     ZG_REQUIRE(a.rows * a.segments < 0x7fffffffull, "distill: %zu rows of %u columns", a.rows, a.cols);
-    if (a.cols <= 1024) {
+    if (a.cols <= 512) {
+        ZG_ROWS(64, 2);
+    } else if (a.cols <= 1024) {
         ZG_ROWS(64, 4);
     } else if (a.cols <= 2048) {
         ZG_ROWS(64, 8);
@@ -1524,6 +1533,7 @@ static int distill_launch(zg_hip_ctx* ctx, DistillArgs a, float* loss, bool* sum
     }
 #undef ZG_GRAD
 #undef ZG_ROWS
+#undef ZG_ROWS_
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
 }
