@@ -2947,7 +2947,13 @@ __global__ __launch_bounds__(256) void expert_join_kernel(const float* parts, fl
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     float s = 0.f;
-    for (unsigned p = 0; p < n_parts; p++) s += parts[(size_t)p * n + i];
+    for (unsigned p0 = 0; p0 < n_parts; p0 += 16) {  // sixteen loads in flight
+        float v[16];
+#pragma unroll
+        for (unsigned u = 0; u < 16; u++) v[u] = p0 + u < n_parts ? parts[(size_t)(p0 + u) * n + i] : 0.f;
+#pragma unroll
+        for (unsigned u = 0; u < 16; u++) s += v[u];
+    }
     to[i] = accumulate ? to[i] + s : s;
 }
 }  // namespace zg
@@ -2998,11 +3004,11 @@ ZG_API int zg_hip_expert_linear_bwd(zg_hip_ctx* ctx, const float* gy, const floa
     g.bounded_tail = fan_out % 4 != 0 || fan_in % 4 != 0;
     // few rows: the kernel that writes wide (64 experts of 512 x 512, 512 rows: 28 against 32 us, 1024 rows: 44 against 34)
     const bool few = n_rows / n_experts <= 8;
-    // 128 x 128 tiles where there are several for every compute unit (16 experts of 2048 x 1024, 16384 rows: 490 us against 548 with
-    // 64 x 64), else the smaller ones (64 experts of 512 x 512, 4096 rows, one expert with 609: 88 us the three products against 96)
+    // 128 x 128 tiles where there are several for every compute unit (the whole backward of 16 experts of 2048 x 1024 over 16384 rows: 1060
+    // us against 1122 with 64 x 64), else the smaller ones (64 experts of 512 x 512, 4096 rows, one expert with 609: 88 us the three products against 96)
     const bool large = n_experts * ceil_div_sz(fan_out, 128) * ceil_div_sz(fan_in, 128) >= 6 * (size_t)ctx->n_cu;
     // An expert's rows in four parts or more, of 128 or more, where the tiles alone leave compute units without one (the whole backward of
-    // 1024 -> 64 for 4000 rows of one expert: 46 us against 110, of 64 -> 64 for 16384 rows of four: 45 against 198).  Two or three parts
+    // 1024 -> 64 for 4000 rows of one expert: 35 us against 110, of 64 -> 64 for 16384 rows of four: 31 against 198).  Two or three parts
     // do not pay for the launch that adds them up (256 -> 256, 300 rows: 22 us against 21).
     const size_t tiles = n_experts * ceil_div_sz(fan_out, 64) * ceil_div_sz(fan_in, 64), n_weights = n_experts * fan_out * fan_in;
     size_t w_parts = few || tiles >= (size_t)ctx->n_cu ? 1 : 2 * (size_t)ctx->n_cu / tiles;
@@ -3010,10 +3016,11 @@ ZG_API int zg_hip_expert_linear_bwd(zg_hip_ctx* ctx, const float* gy, const floa
     if (w_parts < 4) w_parts = 1;
     // workspace: the experts' order, the parts of the weight gradient, those of the bias gradient
     const size_t order_bytes = n_experts > kWave && !few ? (n_experts * sizeof(uint32_t) + 255) / 256 * 256 : 0;
-    size_t parts = 1;  // about 128 rows of an average expert each
-    if (gb) parts = n_rows / (n_experts * 128);
+    // parts of the bias gradient: about 32 rows of an average expert (the whole backward of 16 experts of 2048 x 1024 over 16384
+    // rows: 1047 us, with parts of 128 rows 1065), but none when they would be fewer than four, for which the second launch does not pay
+    size_t parts = gb ? n_rows / (n_experts * 32) : 1;
     if (parts > 64) parts = 64;
-    if (parts < 1) parts = 1;
+    if (parts < 4) parts = 1;
     const size_t w_bytes = w_parts > 1 ? (w_parts * n_weights * sizeof(float) + 255) / 256 * 256 : 0;
     const size_t need = order_bytes + w_bytes + (gb && parts > 1 ? parts * n_experts * fan_out * sizeof(float) : 0);
     char* ws = nullptr;
