@@ -3007,12 +3007,14 @@ ZG_API int zg_hip_expert_linear_bwd(zg_hip_ctx* ctx, const float* gy, const floa
     // 128 x 128 tiles where there are several for every compute unit (the whole backward of 16 experts of 2048 x 1024 over 16384 rows: 1060
     // us against 1122 with 64 x 64), else the smaller ones (64 experts of 512 x 512, 4096 rows, one expert with 609: 88 us the three products against 96)
     const bool large = n_experts * ceil_div_sz(fan_out, 128) * ceil_div_sz(fan_in, 128) >= 6 * (size_t)ctx->n_cu;
-    // An expert's rows in four parts or more, of 128 or more, where the tiles alone leave compute units without one (the whole backward of
-    // 1024 -> 64 for 4000 rows of one expert: 35 us against 110, of 64 -> 64 for 16384 rows of four: 31 against 198).  Two or three parts
-    // do not pay for the launch that adds them up (256 -> 256, 300 rows: 22 us against 21).
+    // An expert's rows in four parts or more where there are fewer than two tiles for every compute unit, four then: up to 16 parts of
+    // 32 rows of an average expert, more only of 128 rows (the whole backward of 1024 -> 64 for 4000 rows of one expert: 35 us against
+    // 110, of 64 -> 64 for 16384 rows of four: 31 against 198, of 100 -> 100 for 10000 rows of 64, one with 1300: 45 against 59; of 200
+    // -> 200 for 3000 rows of 16: 36 against 34).  Two or three parts do not pay for the launch that adds them up.
     const size_t tiles = n_experts * ceil_div_sz(fan_out, 64) * ceil_div_sz(fan_in, 64), n_weights = n_experts * fan_out * fan_in;
-    size_t w_parts = few || tiles >= (size_t)ctx->n_cu ? 1 : 2 * (size_t)ctx->n_cu / tiles;
-    if (w_parts > n_rows / (n_experts * 128)) w_parts = n_rows / (n_experts * 128);
+    size_t w_parts = few || tiles >= 2 * (size_t)ctx->n_cu ? 1 : 4 * (size_t)ctx->n_cu / tiles;
+    const size_t short_parts = n_rows / (n_experts * 32) < 16 ? n_rows / (n_experts * 32) : 16, long_parts = n_rows / (n_experts * 128);
+    if (w_parts > short_parts && w_parts > long_parts) w_parts = short_parts > long_parts ? short_parts : long_parts;
     if (w_parts < 4) w_parts = 1;
     // workspace: the experts' order, the parts of the weight gradient, those of the bias gradient
     const size_t order_bytes = n_experts > kWave && !few ? (n_experts * sizeof(uint32_t) + 255) / 256 * 256 : 0;
