@@ -58,8 +58,8 @@ int zg_hip_distill_fwd(zg_hip_ctx *ctx, const float *logits, const float *teache
 int zg_hip_distill_bwd(zg_hip_ctx *ctx, const float *logits, const float *teacher, const uint64_t *indices,
                        const float *row_weights, const float *stats, float *grad, size_t rows, size_t cols, size_t k,
                        float temperature, int accumulate);
-/* forward and the backward of the scalar loss (upstream gradient 1) in one call; the row is read once where it fits in a
- * workgroup's registers */
+/* forward and the backward of the scalar loss (upstream gradient 1) in one call; rows of up to 65536 columns are read once,
+ * longer ones twice */
 int zg_hip_distill_fwd_bwd(zg_hip_ctx *ctx, const float *logits, const float *teacher, const uint64_t *indices,
                            const float *row_weights, float *stats, float *row_loss, float *loss, float *grad, size_t rows,
                            size_t cols, size_t k, float temperature, int accumulate);
