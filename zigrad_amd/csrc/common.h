@@ -445,6 +445,15 @@ inline size_t mul_sat(size_t a, size_t b) {
     return __builtin_mul_overflow(a, b, &r) ? (size_t)-1 : r;
 }
 
+// A dimension of a launch's grid has fewer than 2^32 threads: the packet that goes to the hardware counts threads in 32 bits, and a
+// longer grid is cut off without an error.
+constexpr size_t most_groups(size_t threads) { return ((size_t)1 << 31) / threads; }
+// n units of work in as many launches as it takes, each of at most `most`: launch(first unit, their number).
+template <class Launch>
+inline void in_launches(size_t n, size_t most, Launch launch) {
+    for (size_t first = 0; first < n; first += most) launch(first, n - first < most ? n - first : most);
+}
+
 // Makes the context's device current for the length of a call (a caller may have another one current).
 struct DeviceGuard {
     int before = -1;

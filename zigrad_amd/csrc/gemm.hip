@@ -226,6 +226,7 @@ struct GemmArgs {
     const uint64_t* offsets;
     const uint32_t* order;  // the experts, those with most rows first (null with at most 64: the workgroups find out themselves)
     unsigned n_experts;
+    unsigned first_group;  // workgroups in the launches before this one
     size_t n_rows;
 };
 
@@ -373,8 +374,8 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_kernel(GemmArgs g) {
         // tiles there really are, dealt to the XCDs in contiguous runs; the grid has room for the most there can be
         const unsigned tiles_m = expert_tiles<BM>(g.offsets, g.n_experts, g.n_rows, threadIdx.x & 63);
         const unsigned total = tiles_m * g.tiles_n, run = (total + 7) / 8;
-        const unsigned id = (blockIdx.x & 7u) * run + (blockIdx.x >> 3);
-        if ((blockIdx.x >> 3) >= run || id >= total) return;
+        const unsigned group = g.first_group + blockIdx.x, id = (group & 7u) * run + (group >> 3);
+        if ((group >> 3) >= run || id >= total) return;
         tile_coords(id, tiles_m, g.tiles_n, tm, tn);
         const ExpertTile t = find_expert_tile<BM>(g.offsets, g.n_experts, g.n_rows, tm, threadIdx.x & 63);
         tm = t.tile;
@@ -1549,6 +1550,7 @@ static GemmArgs gemm_args(const float* A, const float* B, float* C, size_t m, si
     g.offsets = nullptr;
     g.order = nullptr;
     g.n_experts = 0;
+    g.first_group = 0;
     g.n_rows = 0;
     return g;
 }
@@ -2617,7 +2619,7 @@ __global__ __launch_bounds__(256) void expert_few_kernel(GemmArgs g) {
     typedef float piece4 __attribute__((ext_vector_type(4), aligned(4)));
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int r = lane & 15, q = lane >> 4;
-    const unsigned tile_m = blockIdx.x / g.tiles_n, tn = blockIdx.x % g.tiles_n;
+    const unsigned group = g.first_group + blockIdx.x, tile_m = group / g.tiles_n, tn = group % g.tiles_n;
     if (tile_m >= expert_tiles<16 * RB>(g.offsets, g.n_experts, g.n_rows, lane)) return;
     const ExpertTile t = find_expert_tile<16 * RB>(g.offsets, g.n_experts, g.n_rows, tile_m, lane);
     const unsigned left = t.count - t.tile * 16 * RB, rows = left < 16 * RB ? left : 16 * RB;  // of this tile
@@ -2726,7 +2728,10 @@ static int launch_expert_few(zg_hip_ctx* ctx, GemmArgs g) {
     g.tiles_n = (unsigned)ceil_div_sz(g.N, 16 * CB);
     const size_t most = g.n_rows / (16 * RB) + (g.n_rows < g.n_experts ? g.n_rows : g.n_experts);
     ZG_REQUIRE(most * g.tiles_n < 0x7fffffffull, "expert_linear: %zu workgroups", most * g.tiles_n);
-    hipLaunchKernelGGL((expert_few_kernel<RB, CB, BATCH, B_KMAJOR>), dim3((unsigned)(most * g.tiles_n)), dim3(256), 0, ctx->stream, g);
+    in_launches(most * g.tiles_n, most_groups(256), [&](size_t first, size_t n) {
+        g.first_group = (unsigned)first;
+        hipLaunchKernelGGL((expert_few_kernel<RB, CB, BATCH, B_KMAJOR>), dim3((unsigned)n), dim3(256), 0, ctx->stream, g);
+    });
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
 }
@@ -2739,8 +2744,10 @@ static int launch_expert_rows(zg_hip_ctx* ctx, GemmArgs g) {
     const size_t blocks = (most * g.tiles_n + 7) / 8 * 8;
     ZG_REQUIRE(blocks < 0x7fffffffull, "expert_linear: %zu workgroups", blocks);
     constexpr size_t lds = 2 * (size_t)(Tile<BM, true>::ELEMS + Tile<BN, B_KMAJOR>::ELEMS) * sizeof(float);
-    hipLaunchKernelGGL((gemm_kernel<BM, BN, true, B_KMAJOR, 1, false, 1>), dim3((unsigned)blocks), dim3(kGemmThreads), lds,
-                       ctx->stream, g);
+    in_launches(blocks, most_groups(kGemmThreads), [&](size_t first, size_t n) {  // (whole rounds of the XCDs each)
+        g.first_group = (unsigned)first;
+        hipLaunchKernelGGL((gemm_kernel<BM, BN, true, B_KMAJOR, 1, false, 1>), dim3((unsigned)n), dim3(kGemmThreads), lds, ctx->stream, g);
+    });
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
 }
@@ -2786,7 +2793,7 @@ template <int BM, int BN>
 static int launch_expert_weights(zg_hip_ctx* ctx, GemmArgs g, unsigned parts) {
     g.tiles_m = (unsigned)ceil_div_sz(g.M, BM);
     g.tiles_n = (unsigned)ceil_div_sz(g.N, BN);
-    ZG_REQUIRE((size_t)g.tiles_m * g.tiles_n < 0x7fffffffull, "expert_linear_bwd: a layer of %zu x %zu", g.M, g.N);
+    ZG_REQUIRE((size_t)g.tiles_m * g.tiles_n <= most_groups(kGemmThreads), "expert_linear_bwd: a layer of %zu x %zu", g.M, g.N);
     constexpr size_t lds = 2 * (size_t)(Tile<BM, false>::ELEMS + Tile<BN, false>::ELEMS) * sizeof(float);
     hipLaunchKernelGGL((gemm_kernel<BM, BN, false, false, 1, false, 2>), dim3(g.tiles_m * g.tiles_n, parts, g.n_experts),
                        dim3(kGemmThreads), lds, ctx->stream, g);

@@ -834,6 +834,19 @@ struct DistillArgs {
     float temp, inv_temp, scale, mean;  // scale = log2(e) / temp
     uint32_t segments, segment;         // the gradient alone: parts of a row, and their columns
     bool once;                          // more is read than the memory-side cache holds: loads leave nothing there
+
+    DistillArgs part(size_t first, size_t n) const {  // n rows from `first` on
+        DistillArgs a = *this;
+        a.x += first * cols;
+        a.t += first * k;
+        a.idx += first * k;
+        if (w) a.w += first;
+        a.stats += 2 * first;
+        if (row_loss) a.row_loss += first;
+        if (grad) a.grad += first * cols;
+        a.rows = n;
+        return a;
+    }
 };
 
 // Loads that pass by the memory-side cache (256 MB) win as soon as it can not hold what is read (logits, an old gradient: 16384 x
@@ -1474,20 +1487,28 @@ static int distill_launch(zg_hip_ctx* ctx, DistillArgs a, float* loss, bool* sum
         ZG_LAUNCH_CHECK();
         return ZG_HIP_OK;
     }
-#define ZG_ROWS_(NT, VPT, ENTRIES)                                                                                                          \
-    hipLaunchKernelGGL((distill_row_kernel<NT, VPT, ENTRIES, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(a.rows, NT < 256 ? 256 / NT : 1)), \
-                       dim3(NT < 256 ? 256 : NT), 0, ctx->stream, a)
+    // The rows of a launch but the last are a multiple of 32 (a segment has 8192 columns of fewer than 2^31): the gradient's pieces begin
+    // where they would in one launch.
+#define ZG_ROWS_(NT, VPT, ENTRIES)                                                                                                        \
+    do {                                                                                                                                  \
+        constexpr size_t threads = NT < 256 ? 256 : NT, per = threads / NT;                                                               \
+        in_launches(a.rows, most_groups(threads) * per, [&](size_t first, size_t n) {                                                     \
+            hipLaunchKernelGGL((distill_row_kernel<NT, VPT, ENTRIES, FWD, BWD, ACC>), dim3((unsigned)ceil_div_sz(n, per)), dim3(threads), \
+                               0, ctx->stream, a.part(first, n));                                                                         \
+        });                                                                                                                               \
+    } while (0)
 #define ZG_ROWS(NT, VPT)                                       \
     do {                                                       \
         if (a.k <= NT && few) ZG_ROWS_(NT, VPT, 1);            \
         else ZG_ROWS_(NT, VPT, (kMaxK + NT - 1) / NT);         \
     } while (0)
 #define ZG_GRAD(NT, R, L)                                                                                                              \
-    do {                                                                                                                               \
-        const dim3 grid((unsigned)(a.rows * a.segments));                                                                              \
-        if (a.once) hipLaunchKernelGGL((distill_grad_kernel<NT, R, L, FWD, ACC, true>), grid, dim3(NT), 0, ctx->stream, a);            \
-        else hipLaunchKernelGGL((distill_grad_kernel<NT, R, L, FWD, ACC, false>), grid, dim3(NT), 0, ctx->stream, a);                  \
-    } while (0)
+    in_launches(a.rows, most_groups(NT) / a.segments / 32 * 32, [&](size_t first, size_t n) {                                          \
+        const dim3 grid((unsigned)(n * a.segments));                                                                                   \
+        const DistillArgs part = a.part(first, n);                                                                                     \
+        if (a.once) hipLaunchKernelGGL((distill_grad_kernel<NT, R, L, FWD, ACC, true>), grid, dim3(NT), 0, ctx->stream, part);         \
+        else hipLaunchKernelGGL((distill_grad_kernel<NT, R, L, FWD, ACC, false>), grid, dim3(NT), 0, ctx->stream, part);               \
+    })
     // One entry of the teacher a thread where that does (65536 rows of 600, k = 8: step 55 us against 78 with room for 512), but for the
     // gradient that is added to in rows of more than 1024 columns (2000, k = 64: 300 us against 285).
     const bool few = !ACC || a.cols <= 1024;
@@ -1495,7 +1516,6 @@ static int distill_launch(zg_hip_ctx* ctx, DistillArgs a, float* loss, bool* sum
     a.segments = FWD || a.cols <= 8192 ? 1u : (a.cols - 1) / 8192 + 1;
     a.segment = ((a.cols - 1) / a.segments + 4) & ~3u;
     a.segments = (a.cols - 1) / a.segment + 1;  // as many as have columns
-    ZG_REQUIRE(a.rows * a.segments < 0x7fffffffull, "distill: %zu rows of %u columns", a.rows, a.cols);
     if (a.cols <= 512) {
         ZG_ROWS(64, 2);
     } else if (a.cols <= 1024) {
@@ -1604,7 +1624,7 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
         uint32_t n_seg = (uint32_t)ceil_div_sz(cols, kTopkSegment);
         const uint32_t len = (uint32_t)((ceil_div_sz(cols, n_seg) + 3) & ~(size_t)3);  // at most kTopkSegment, as n_seg segments reach
         n_seg = (uint32_t)ceil_div_sz(cols, len);
-        if (cols - (size_t)(n_seg - 1) * len >= k) {
+        if (cols - (size_t)(n_seg - 1) * len >= k && rows * n_seg <= most_groups(256)) {
             uint64_t* keys = (uint64_t*)workspace(ctx, rows * n_seg * k * sizeof(uint64_t));
             if (!keys) return ZG_HIP_EOOM;
             hipLaunchKernelGGL(topk_segments_kernel, dim3((unsigned)(rows * n_seg)), dim3(256), 0, ctx->stream, x, keys, c32, k32, len, n_seg);
@@ -1617,9 +1637,11 @@ ZG_API int zg_hip_topk_fwd(zg_hip_ctx* ctx, const float* x, float* values, uint6
     // A wave per row as far as its 256 groups can bound k and there are rows enough to fill the compute units (or the row is
     // short): its waves never wait for each other (64 of 8192 in 8192 rows: 64 us against 97 us with a workgroup per row).  A
     // workgroup per row else.
-#define ZG_TOPK_SHORT(L, KPL)                                                                                                    \
-    hipLaunchKernelGGL((topk_short_kernel<L, KPL>), dim3((unsigned)ceil_div_sz(rows, 256 / (L))), dim3(256), 0, ctx->stream, x,      \
-                       values, indices, rows, c32, k32)
+#define ZG_TOPK_SHORT(L, KPL)                                                                                                       \
+    in_launches(rows, most_groups(256) * (256 / (L)), [&](size_t first, size_t n) {                                                 \
+        hipLaunchKernelGGL((topk_short_kernel<L, KPL>), dim3((unsigned)ceil_div_sz(n, 256 / (L))), dim3(256), 0, ctx->stream,       \
+                           x + first * cols, values + first * k, indices + first * k, n, c32, k32);                                 \
+    })
     // (8 of 128 in 65536 rows 15 us against 29 by a wave per row, 4 of 200 25 against 26, 8 of 256 34 against 29, 16 of 256 48 against 30)
     if (cols <= 256 && k <= (cols <= 128 ? 16u : 4u)) {
         if (cols <= 16) ZG_TOPK_SHORT(4, 4);
@@ -1670,21 +1692,30 @@ ZG_API int zg_hip_topk_bwd(zg_hip_ctx* ctx, const uint64_t* indices, const float
         hipLaunchKernelGGL(topk_bwd_add_kernel, dim3(row_grid(ceil_div_sz(rows, 4 * per_wave))), dim3(256), 0, ctx->stream, indices, y_g,
                            x_g, rows, c32, k32, bits);
     } else if (cols <= 256 && k <= 16) {
-        const dim3 grid((unsigned)ceil_div_sz(rows, 16));
-        if (cols <= 64) hipLaunchKernelGGL(topk_bwd_short_kernel<1>, grid, dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32);
-        else if (cols <= 128) hipLaunchKernelGGL(topk_bwd_short_kernel<2>, grid, dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32);
-        else hipLaunchKernelGGL(topk_bwd_short_kernel<4>, grid, dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32);
+        in_launches(rows, most_groups(256) * 16, [&](size_t first, size_t n) {
+            auto launch = [&](auto* kernel) {
+                hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div_sz(n, 16)), dim3(256), 0, ctx->stream, indices + first * k, y_g + first * k,
+                                   x_g + first * cols, n, c32, k32);
+            };
+            if (cols <= 64) launch(topk_bwd_short_kernel<1>);
+            else if (cols <= 128) launch(topk_bwd_short_kernel<2>);
+            else launch(topk_bwd_short_kernel<4>);
+        });
     } else {
         // even spans of whole 128-byte lines
         const size_t span = cols <= 1024 ? cols : (ceil_div_sz(cols, ceil_div_sz(cols, 4096)) + 31) / 32 * 32;
-        const size_t spans = ceil_div_sz(cols, span), blocks = cols <= 1024 ? ceil_div_sz(rows, 4) : mul_sat(rows, spans);
-        ZG_REQUIRE(blocks < 0x7fffffffull, "topk_bwd: %zu rows of %zu columns", rows, cols);
-        if (cols <= 1024)
-            hipLaunchKernelGGL(topk_bwd_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32,
-                               (uint32_t)spans, (uint32_t)span, bits);
-        else
-            hipLaunchKernelGGL(topk_bwd_kernel<256>, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, indices, y_g, x_g, rows, c32, k32,
-                               (uint32_t)spans, (uint32_t)span, bits < 12 ? bits : 12);
+        const size_t spans = ceil_div_sz(cols, span), most = most_groups(256);
+        in_launches(rows, cols <= 1024 ? most * 4 : most / spans, [&](size_t first, size_t n) {
+            const uint64_t* idx = indices + first * k;
+            const float* g = y_g + first * k;
+            float* out = x_g + first * cols;
+            if (cols <= 1024)
+                hipLaunchKernelGGL(topk_bwd_kernel<64>, dim3((unsigned)ceil_div_sz(n, 4)), dim3(256), 0, ctx->stream, idx, g, out, n, c32, k32,
+                                   (uint32_t)spans, (uint32_t)span, bits);
+            else
+                hipLaunchKernelGGL(topk_bwd_kernel<256>, dim3((unsigned)(n * spans)), dim3(256), 0, ctx->stream, idx, g, out, n, c32, k32,
+                                   (uint32_t)spans, (uint32_t)span, bits < 12 ? bits : 12);
+        });
     }
     ZG_LAUNCH_CHECK();
     return ZG_HIP_OK;
