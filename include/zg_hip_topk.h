@@ -96,7 +96,9 @@ int zg_hip_expert_combine_bwd(zg_hip_ctx *ctx, const float *out_g, const float *
  * the experts' Linear layers: zg_hip_linear_fwd and zg_hip_linear_bwd with weights w[e, fan_out, fan_in] and bias[e, fan_out]
  * for the rows offsets[e] .. offsets[e + 1] - 1 (as zg_hip_expert_sort leaves them in device memory: the host never needs the
  * counts).  Rows behind offsets[n_experts] are neither read nor written; offsets beyond n_rows are taken as n_rows and a range that ends
- * before it begins as empty.  n_rows < 2^31, fan_in and fan_out < 2^21, n_experts <= ZG_HIP_EXPERTS_MAX.
+ * before it begins as empty.  The ranges must not overlap, which offsets that never decrease can not: where they do, what the rows of y and
+ * gx in the overlapping ranges hold afterwards is undefined (gw_e and gb_e are sums over expert e's range all the same, and nothing
+ * outside the ranges is touched).  n_rows < 2^31, fan_in and fan_out < 2^21, n_experts <= ZG_HIP_EXPERTS_MAX.
  *   forward   y = x w_e^T + bias_e (null: none), max(0, .) when relu
  *   backward  gw_e += gy_e^T x_e;  gb_e += column sums of gy_e (null: none);  gx = gy w_e, zero where act_in <= 0 (gx null: no
  *             input gradient, w is not read; act_in null: no mask).  accumulate == 0: gw and gb are written, zero for an
