@@ -723,11 +723,10 @@ __device__ __forceinline__ uint64_t same_lanes(uint32_t v, int bits, uint64_t am
     return among;
 }
 // Adds the entries of a wave to a row, one a lane: `same`, the lanes that name this lane's column (none: no entry); the lowest of them
-// writes, the gradients in the order of the lanes.  FRESH: nothing is there yet.
-template <bool FRESH>
+// writes, the gradients in the order of the lanes.
 __device__ __forceinline__ void add_entries(float* at, float g, uint64_t same, int lane) {
     const bool writes = same != 0 && (same & (((uint64_t)1 << lane) - 1)) == 0;
-    float v = (!FRESH && writes) ? __fadd_rn(*at, g) : g;
+    float v = writes ? __fadd_rn(*at, g) : g;
     uint64_t rest = writes ? same & (same - 1) : 0;
     while (__any(rest != 0)) {
         const int l = rest ? __builtin_ctzll(rest) : lane;
@@ -772,7 +771,7 @@ __global__ __launch_bounds__(256) void topk_bwd_kernel(const uint64_t* indices, 
                 const uint32_t col = here ? (uint32_t)at : 0u;
                 uint64_t same = same_lanes(col, bits, heres);
                 if (!here) same = 0;
-                add_entries<false>(span + col, here ? g : 0.f, same, lane);
+                add_entries(span + col, here ? g : 0.f, same, lane);
                 select_sync<kWave>();
             }
             j0 += kWave;
@@ -805,7 +804,7 @@ __global__ __launch_bounds__(256) void topk_bwd_add_kernel(const uint64_t* indic
             const uint32_t col = here ? (uint32_t)idx : 0u;
             uint64_t same = same_lanes(col, bits, __ballot(here) & row_lanes);
             if (!here) same = 0;
-            add_entries<false>(x_g + (here ? r : 0) * cols + col, here ? y_g[i] : 0.f, same, lane);
+            add_entries(x_g + (here ? r : 0) * cols + col, here ? y_g[i] : 0.f, same, lane);
         }
     }
 }
@@ -1062,7 +1061,7 @@ __device__ __forceinline__ void span_shares(float* span, const uint32_t* col, co
         if (!heres) continue;
         uint64_t same = same_lanes(here ? at : 0u, bits, heres);
         if (!here) same = 0;
-        add_entries<false>(span + (here ? at : 0u), here ? q[j0 + lane] : 0.f, same, lane);
+        add_entries(span + (here ? at : 0u), here ? q[j0 + lane] : 0.f, same, lane);
         select_sync<kWave>();
     }
 }
