@@ -42,7 +42,7 @@ int zg_hip_topk_bwd(zg_hip_ctx *ctx, const uint64_t *indices, const float *y_g, 
  * ZG_HIP_TOPK_MAX_K).  With q = softmax(teacher[r, :] / temperature) over the k kept logits and p = softmax(logits[r, :] /
  * temperature) over all classes:
  *   row_loss[r] = temperature^2 sum_j q_j (log q_j - log p_{indices[r, j]})
- *   loss        = sum_r w_r row_loss[r]              w = row_weights, or 1 / rows each when row_weights is null
+ *   loss        = sum_r w_r row_loss[r]              w = row_weights (finite), or 1 / rows each when row_weights is null
  *   grad[r, c] += w_r temperature (p_c - sum of the q_j whose index is c)      accumulate == 0: grad is written, not read
  * An index that is not below cols is padding: its logit is left out of q.  A row adds exactly nothing (row_loss 0, gradient
  * 0, whatever its logits hold) when its weight is 0, when it has no teacher logit above -inf, or when all its logits
