@@ -3009,7 +3009,9 @@ ZG_API int zg_hip_expert_linear_bwd(zg_hip_ctx* ctx, const float* gy, const floa
     g.split_tiles = (size_t)1 << 28;  // all of k
     g.c_vec = aligned16(gw) && fan_in % 4 == 0;
     g.bounded_tail = fan_out % 4 != 0 || fan_in % 4 != 0;
-    // few rows: the kernel that writes wide (64 experts of 512 x 512, 512 rows: 28 against 32 us, 1024 rows: 44 against 34)
+    // few rows: the kernel that writes wide (64 experts of 512 x 512, 512 rows: 28 against 32 us, 1024 rows: 44 against 34).  The host knows
+    // the average only: with all rows on one expert this kernel walks them one after the other (the whole backward of 256 experts of
+    // 256 x 256, 2048 rows: 426 us against 43 spread evenly), the staged one has them in one part (64 of 512 x 512, 8128 rows: 324 against 104)
     const bool few = n_rows / n_experts <= 8;
     // 128 x 128 tiles where there are several for every compute unit (the whole backward of 16 experts of 2048 x 1024 over 16384 rows: 1060
     // us against 1122 with 64 x 64), else the smaller ones (64 experts of 512 x 512, 4096 rows, one expert with 609: 88 us the three products against 96)

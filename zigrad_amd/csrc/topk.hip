@@ -295,7 +295,8 @@ __device__ __forceinline__ uint32_t select_thin(Select<NT, SEG>& s, Place& at, u
     return t;
 }
 
-// The row again, NT x 4 values at a time, with room made before each.
+// The row again, NT x 4 values at a time, with room made before each.  (64 of 32000 in 8192 rows, 179 us where this is not needed: rows in
+// rising order 2150 us, one number in a hundred among zeros 370, four different values 273.)
 template <int NT, int SEG>
 __device__ void select_slowly(Select<NT, SEG>& s, Place& at, const float* row, uint32_t cols, uint32_t k) {
     const uint32_t whole = cols & ~3u;
@@ -815,7 +816,7 @@ __global__ __launch_bounds__(256) void topk_bwd_add_kernel(const uint64_t* indic
 //   row_loss = T^2 (sum_j f_j ((t_j - tm) - (x_{i_j} - m)) / T / S - log S + log s)
 // A row's logits are read once, into registers, by 16 lanes, a wave, or a workgroup of 256, 512 or 1024, by its length (the loss alone
 // reads rows of more than 32768 columns with a running maximum; for more than 65536 the gradient reads them again); the maxima, then
-// all sums, take one reduction each.  Bound by memory: 8192 x 32000 forward 155 us, 6.8 TB/s.  In the gradient of rows of up to 2048
+// all sums, take one reduction each.  Bound by memory: 8192 x 32000 forward 159 us, 6.6 TB/s.  In the gradient of rows of up to 2048
 // columns the q_j go into a stretch of LDS laid out like the row, from where every thread takes what belongs to its columns; of longer
 // rows the few classes that have a share are written a second time.  Either way a class that is named twice gets both shares,
 // added in the order of j.
@@ -1542,8 +1543,8 @@ static int distill_launch(zg_hip_ctx* ctx, DistillArgs a, float* loss, bool* sum
         } else if (a.cols <= 65536) {
             ZG_GRAD(1024, 16, 0);
         } else {
-            // Rows that no workgroup holds: the loss, then the gradient.  (2048 x 128000: 560 us, one kernel that read each row twice
-            // 526; 16 x 128000: 23 us against 36.  Some rows at a time, for the second pass to find them in the memory-side cache,
+            // Rows that no workgroup holds: the loss, then the gradient.  (2048 x 128000: 514 us, 16 x 128000: 18 us; one kernel that read
+            // each row twice took 526 and 36.  Some rows at a time, for the second pass to find them in the memory-side cache,
             // costs more in half-empty launches than it saves: 619 us.)
             bool unused;
             if (int rc = distill_launch<true, false, false>(ctx, a, loss, &unused)) return rc;
